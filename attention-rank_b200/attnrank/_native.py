@@ -18,6 +18,7 @@ AR_ERR_DEVICE = 3
 AR_ERR_INTERNAL = 4
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+ROPE_NONE, ROPE_LINEAR, ROPE_BANDS, ROPE_YARN = 0, 1, 2, 3
 KERNEL_CLASS_COUNT = 12  # AR_KERNEL_CLASS_COUNT
 
 
@@ -83,6 +84,43 @@ class BasinStatsStruct(ctypes.Structure):
     ]
 
 
+class RopeScalingStruct(ctypes.Structure):
+    _fields_ = [
+        ("theta", ctypes.c_float),
+        ("rotary_dim", ctypes.c_int),
+        ("kind", ctypes.c_int),
+        ("factor", ctypes.c_float),
+        ("low", ctypes.c_float),
+        ("high", ctypes.c_float),
+        ("original_positions", ctypes.c_int),
+        ("attention_factor", ctypes.c_float),
+    ]
+
+
+class PagedCacheStruct(ctypes.Structure):
+    _fields_ = [
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("page_count", ctypes.c_int),
+        ("page_size", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("dtype", ctypes.c_int),
+    ]
+
+
+class PagedBatchStruct(ctypes.Structure):
+    _fields_ = [
+        ("sequence_count", ctypes.c_int),
+        ("token_count", ctypes.c_int),
+        ("max_query_tokens", ctypes.c_int),
+        ("page_table_stride", ctypes.c_int),
+        ("q_offsets", ctypes.c_void_p),
+        ("kv_lengths", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
@@ -133,6 +171,14 @@ SIGNATURES: dict[str, list] = {
     "ar_decode_gemv": [_P, _P, _I, _I, _P, _I, _I, _P],
     "ar_decode_gate_up": [_P, _P, _I, _I, _P, _I, _P],
     "ar_decode_attention": [_P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _I, _P],
+    "ar_rope_frequencies": [ctypes.POINTER(RopeScalingStruct), _P, _P],
+    "ar_rope_table_scaled": [ctypes.POINTER(RopeScalingStruct), _I, _P, _P, _P],
+    "ar_rotary_positions": [_P, _I64, _I64, _P, _I64, _I64, _P, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P, _I, _P],
+    "ar_paged_append": [ctypes.POINTER(PagedCacheStruct), ctypes.POINTER(PagedBatchStruct), _P, _I64, _P, _I, _P, _I64,
+                        _P, _P, _I, _I, _I, _P, _P],
+    "ar_paged_attention_workspace": [ctypes.POINTER(PagedCacheStruct), ctypes.POINTER(PagedBatchStruct), _I],
+    "ar_paged_attention": [ctypes.POINTER(PagedCacheStruct), ctypes.POINTER(PagedBatchStruct), _P, _I64, _I, _F, _I, _P,
+                           _I64, _P, _P, _I64, _P, _P],
     "ar_bounded_wait_selftest": [_I, ctypes.c_uint32, _P],
     "ar_profile_from_accumulated": [_P, _I, _I64, _P, _P],
     "ar_position_order": [_P, _I, _P],
@@ -147,6 +193,7 @@ _RESTYPES = {
     "ar_prepared_scan_destroy": None,
     "ar_sampler_destroy": None,
     "ar_prepared_scan_bytes": ctypes.c_int64,
+    "ar_paged_attention_workspace": ctypes.c_int64,
     "ar_kernel_class_name": ctypes.c_char_p,
     "ar_engine_stream": ctypes.c_void_p,
     "ar_engine_device": ctypes.c_int,

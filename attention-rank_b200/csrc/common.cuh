@@ -19,6 +19,7 @@ enum DeviceStatus : int {
   kStatusTokenOutOfRange = 1,   // a token id outside [0, vocab)
   kStatusPositionOutOfRange = 2,  // a RoPE position beyond the cos/sin table
   kStatusWaitTimeout = 3,       // an mbarrier wait exceeded its iteration limit
+  kStatusPagedBatch = 4,        // offsets, lengths or page ids of a paged batch outside their arrays
 };
 
 __device__ __forceinline__ void report_status(int* status, int code) {

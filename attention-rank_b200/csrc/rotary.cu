@@ -1,0 +1,250 @@
+// Rotary positions: cos/sin tables scaled for long contexts, and the rotation of part of a head in
+// the half or the interleaved layout (contracts in include/attnrank_b200.h).
+//
+// Table: the angle p f is formed in turns, p (f / 2 pi), in fp64 (an fp32 product loses all digits
+// of the fraction near 2^24 turns and is off by 1e-3 rad at 1e4), reduced to its nearest whole turn
+// in fp64, and only the remainder in [-1/2, 1/2] turns goes to fp32 and sincospi. Three fp64
+// operations a value, so the kernel is bound by the 8 bytes it writes for each.
+//
+// Rotation: y_a = a c - b s, y_b = b c + a s, one read and one write of each 16-bit value.
+#include <algorithm>
+
+#include "common.cuh"
+#include "layer_kernels.h"
+#include "paged.h"
+
+namespace arb {
+namespace {
+
+constexpr int kThreads = 256;
+
+__global__ void __launch_bounds__(kThreads) rope_table_scaled_kernel(const __grid_constant__ TableTurns turns, int half,
+                                                                     float multiplier, int64_t values,
+                                                                     float* __restrict__ cos_table,
+                                                                     float* __restrict__ sin_table) {
+  __shared__ double turn[kMaxTableFrequencies];
+  for (int i = threadIdx.x; i < half; i += kThreads) turn[i] = turns.value[i];
+  __syncthreads();
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads * 4;
+  for (int64_t at = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * 4; at < values; at += stride) {
+    int position = static_cast<int>(at / half);
+    int column = static_cast<int>(at - static_cast<int64_t>(position) * half);
+    float c[4], s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const double turned = static_cast<double>(position) * turn[column];
+      const float rest = static_cast<float>(turned - rint(turned));
+      sincospif(2.0f * rest, &s[i], &c[i]);
+      s[i] *= multiplier;
+      c[i] *= multiplier;
+      if (++column == half) {
+        column = 0;
+        ++position;
+      }
+    }
+    if (at + 4 <= values) {
+      __stcs(reinterpret_cast<float4*>(cos_table + at), make_float4(c[0], c[1], c[2], c[3]));
+      __stcs(reinterpret_cast<float4*>(sin_table + at), make_float4(s[0], s[1], s[2], s[3]));
+    } else {
+      for (int i = 0; i < static_cast<int>(values - at); ++i) {
+        cos_table[at + i] = c[i];
+        sin_table[at + i] = s[i];
+      }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v) {
+  return static_cast<float>(v);
+}
+
+// Vector form: an item is one token, kHeads heads and one unit of 16 values of each: eight rotation
+// pairs, or sixteen values behind the rotated part.
+template <typename T, bool kInterleaved, int kHeads>
+__global__ void __launch_bounds__(kThreads) rotary_positions_kernel(const RotaryArgs a, int units, int rotated_units,
+                                                                    int groups, int64_t items) {
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (item >= items) return;
+  const int unit = static_cast<int>(item % units);
+  const int64_t rest = item / units;
+  const int group = static_cast<int>(rest % groups);
+  const int token = static_cast<int>(rest / groups);
+  const int position = __ldg(a.positions + token);
+  if (position < 0 || position >= a.table_positions) {
+    report_status(a.status, kStatusPositionOutOfRange);
+    return;
+  }
+  const bool rotated = unit < rotated_units;
+  int low_at, high_at;
+  if (!rotated) {
+    low_at = a.rotary_dim + (unit - rotated_units) * 16;
+    high_at = low_at + 8;
+  } else if (kInterleaved) {
+    low_at = unit * 16;
+    high_at = low_at + 8;
+  } else {
+    low_at = unit * 8;
+    high_at = (a.rotary_dim >> 1) + unit * 8;
+  }
+  const bool high_in = high_at < a.head_dim;
+  const int first = group * kHeads;
+  const T* x = static_cast<const T*>(a.x) + token * a.x_token_stride;
+  T* out = static_cast<T*>(a.out) + token * a.out_token_stride;
+  uint4 low[kHeads], high[kHeads];
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    if (first + h < a.heads) {
+      const T* row = x + (first + h) * a.x_head_stride;
+      low[h] = *reinterpret_cast<const uint4*>(row + low_at);
+      if (high_in) high[h] = *reinterpret_cast<const uint4*>(row + high_at);
+    }
+  }
+  float c[8], s[8];
+  if (rotated) {
+    const int64_t at = static_cast<int64_t>(position) * (a.rotary_dim >> 1) + unit * 8;
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      const float4 c4 = __ldg(reinterpret_cast<const float4*>(a.cos_table + at + i));
+      const float4 s4 = __ldg(reinterpret_cast<const float4*>(a.sin_table + at + i));
+      c[i] = c4.x, c[i + 1] = c4.y, c[i + 2] = c4.z, c[i + 3] = c4.w;
+      s[i] = s4.x, s[i + 1] = s4.y, s[i + 2] = s4.z, s[i + 3] = s4.w;
+    }
+    if (a.inverse) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] = -s[i];
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    if (first + h >= a.heads) break;
+    if (rotated) rotate16<T, kInterleaved>(low[h], high[h], c, s);
+    T* row = out + (first + h) * a.out_head_stride;
+    *reinterpret_cast<uint4*>(row + low_at) = low[h];
+    if (high_in) *reinterpret_cast<uint4*>(row + high_at) = high[h];
+  }
+}
+
+// Form for sizes, strides or addresses that do not hold 16-byte accesses: an item is one token,
+// kHeads heads and one rotation pair, or two values behind the rotated part.
+template <typename T, bool kInterleaved, int kHeads>
+__global__ void __launch_bounds__(kThreads) rotary_positions_pairs_kernel(const RotaryArgs a, int units,
+                                                                          int rotated_units, int groups,
+                                                                          int64_t items) {
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (item >= items) return;
+  const int unit = static_cast<int>(item % units);
+  const int64_t rest = item / units;
+  const int group = static_cast<int>(rest % groups);
+  const int token = static_cast<int>(rest / groups);
+  const int position = __ldg(a.positions + token);
+  if (position < 0 || position >= a.table_positions) {
+    report_status(a.status, kStatusPositionOutOfRange);
+    return;
+  }
+  const bool rotated = unit < rotated_units;
+  int low_at, high_at;
+  if (!rotated) {
+    low_at = a.rotary_dim + (unit - rotated_units) * 2;
+    high_at = low_at + 1;
+  } else if (kInterleaved) {
+    low_at = unit * 2;
+    high_at = low_at + 1;
+  } else {
+    low_at = unit;
+    high_at = rotated_units + unit;
+  }
+  const bool high_in = high_at < a.head_dim;
+  const int first = group * kHeads;
+  const T* x = static_cast<const T*>(a.x) + token * a.x_token_stride;
+  T* out = static_cast<T*>(a.out) + token * a.out_token_stride;
+  T low[kHeads], high[kHeads];
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    if (first + h < a.heads) {
+      const T* row = x + (first + h) * a.x_head_stride;
+      low[h] = row[low_at];
+      if (high_in) high[h] = row[high_at];
+    }
+  }
+  float c = 1.0f, s = 0.0f;
+  if (rotated) {
+    const int64_t at = static_cast<int64_t>(position) * rotated_units + unit;
+    c = __ldg(a.cos_table + at);
+    s = __ldg(a.sin_table + at);
+    if (a.inverse) s = -s;
+  }
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    if (first + h >= a.heads) break;
+    T* row = out + (first + h) * a.out_head_stride;
+    if (rotated) {
+      const float l = to_float(low[h]);
+      const float r = to_float(high[h]);
+      low[h] = static_cast<T>(l * c - r * s);
+      high[h] = static_cast<T>(r * c + l * s);
+    }
+    row[low_at] = low[h];
+    if (high_in) row[high_at] = high[h];
+  }
+}
+
+template <typename T, bool kInterleaved>
+void launch_layout(const RotaryArgs& a, cudaStream_t stream) {
+  const uintptr_t addresses = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.out) |
+                              reinterpret_cast<uintptr_t>(a.cos_table) | reinterpret_cast<uintptr_t>(a.sin_table);
+  const int64_t strides = a.x_token_stride | a.x_head_stride | a.out_token_stride | a.out_head_stride;
+  const bool vectors = addresses % 16 == 0 && strides % 8 == 0 && a.head_dim % 8 == 0 && a.rotary_dim % 16 == 0;
+  const bool in_place = a.out == a.x;  // the values behind the rotated part are there already
+  const int width = vectors ? 16 : 2;
+  const int rotated_units = a.rotary_dim / width;
+  const int units = in_place ? rotated_units : rotated_units + (a.head_dim - a.rotary_dim + width - 1) / width;
+  auto run = [&](auto kernel, int heads_per_item) {
+    const int groups = (a.heads + heads_per_item - 1) / heads_per_item;
+    const int64_t per_token = static_cast<int64_t>(groups) * units;
+    const int step = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(a.tokens, (int64_t{1} << 30) / per_token)));
+    for (int begin = 0; begin < a.tokens; begin += step) {  // one launch but for batches beyond 2^30 items
+      RotaryArgs part = a;
+      part.tokens = std::min(step, a.tokens - begin);
+      part.x = static_cast<const T*>(a.x) + begin * a.x_token_stride;
+      part.out = static_cast<T*>(a.out) + begin * a.out_token_stride;
+      part.positions = a.positions + begin;
+      const int64_t items = part.tokens * per_token;
+      kernel<<<static_cast<unsigned>((items + kThreads - 1) / kThreads), kThreads, 0, stream>>>(
+          part, units, rotated_units, groups, items);
+    }
+  };
+  // one head an item while that does not fill the GPU, four (one read of cos and sin for them) above
+  const bool few = static_cast<int64_t>(a.tokens) * a.heads * units <= static_cast<int64_t>(sm_count()) * kThreads * 4;
+  if (vectors) {
+    few ? run(rotary_positions_kernel<T, kInterleaved, 1>, 1) : run(rotary_positions_kernel<T, kInterleaved, 4>, 4);
+  } else {
+    few ? run(rotary_positions_pairs_kernel<T, kInterleaved, 1>, 1)
+        : run(rotary_positions_pairs_kernel<T, kInterleaved, 4>, 4);
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_rope_table_scaled(const TableTurns& turns, int half, float multiplier, int positions,
+                                     float* cos_table, float* sin_table, cudaStream_t stream) {
+  if (positions <= 0) return cudaSuccess;
+  const int64_t values = static_cast<int64_t>(positions) * half;
+  const int64_t blocks = (values + kThreads * 4 - 1) / (kThreads * 4);
+  const int grid = static_cast<int>(std::min<int64_t>(blocks, static_cast<int64_t>(sm_count()) * 8));
+  rope_table_scaled_kernel<<<grid, kThreads, 0, stream>>>(turns, half, multiplier, values, cos_table, sin_table);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_rotary_positions(const RotaryArgs& args, cudaStream_t stream) {
+  if (args.tokens <= 0 || args.heads <= 0) return cudaSuccess;
+  if (args.dtype == kActFp16) {
+    args.interleaved ? launch_layout<__half, true>(args, stream) : launch_layout<__half, false>(args, stream);
+  } else {
+    args.interleaved ? launch_layout<__nv_bfloat16, true>(args, stream)
+                     : launch_layout<__nv_bfloat16, false>(args, stream);
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace arb

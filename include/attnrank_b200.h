@@ -302,6 +302,136 @@ int ar_decode_attention(const void* q, const void* k_cache, const void* v_cache,
                         int query_heads, int kv_heads, int head_dim, int sliding_window, void* out, int dtype,
                         void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Serving operators: rotary positions for long contexts, and a paged KV cache with the attention
+ * that reads it. No counterpart in the reference, whose generation keeps one contiguous fp32 cache
+ * per prompt and rotates with one unscaled table (kernels.cu:85-115, model.cu:426-440). They let
+ * many prompts be prefilled in chunks and answered together. Device pointers, asynchronous on
+ * `stream`; a call runs on the device that holds its arrays, whichever is current (stream NULL: that
+ * device's default stream). No call allocates or synchronises, so every one may be captured into a
+ * CUDA graph; lengths, offsets and page ids are read on the device when the work runs.
+ * ------------------------------------------------------------------------------------------ */
+
+/* How the frequencies theta^(-2i/r), i < r/2, r = rotary_dim, are stretched for contexts longer
+ * than the trained window. `original_positions` = L is the trained window, s = factor:
+ *   AR_ROPE_NONE    f_i                      AR_ROPE_LINEAR  f_i / s
+ *   AR_ROPE_BANDS   with t = L f_i / 2 pi turns over the window: t <= low: f_i / s; t >= high: f_i;
+ *                   between them m f_i + (1 - m) f_i / s, m = (t - low) / (high - low)
+ *   AR_ROPE_YARN    with c(b) = r ln(L / (2 pi b)) / (2 ln theta), a = max(floor(c(high)), 0),
+ *                   b = min(ceil(c(low)), r - 1), g = clamp((i - a) / max(b - a, 0.001), 0, 1):
+ *                   g f_i / s + (1 - g) f_i; cos and sin are multiplied by 0.1 ln(s) + 1.
+ * attention_factor, where it is not 0, replaces that multiplier (1 for the other kinds).
+ * theta > 1, finite; rotary_dim even, 2..512; for LINEAR, BANDS and YARN s >= 1; for BANDS and
+ * YARN L >= 1 and 0 < low < high. */
+#define AR_ROPE_NONE 0
+#define AR_ROPE_LINEAR 1
+#define AR_ROPE_BANDS 2
+#define AR_ROPE_YARN 3
+typedef struct {
+  float theta;
+  int rotary_dim;
+  int kind;
+  float factor;
+  float low;
+  float high;
+  int original_positions;
+  float attention_factor;
+} ar_rope_scaling;
+
+/* Host: the scaled frequencies (radians a position, fp64 [rotary_dim / 2]) and the multiplier of
+ * cos and sin (nullable). */
+int ar_rope_frequencies(const ar_rope_scaling* scaling, double* frequencies_out, double* multiplier_out);
+
+/* cos and sin of position * f_i, times the multiplier, fp32 [positions, rotary_dim / 2] each. The
+ * angle is formed and reduced in fp64, so far positions keep their digits. ar_rope_table is the
+ * reference's own fp32 expression; this one is the table of the two operators below. */
+int ar_rope_table_scaled(const ar_rope_scaling* scaling, int positions, float* cos_table, float* sin_table,
+                         void* stream);
+
+/* Rotates the first rotary_dim values of every head of x [token_count][heads][head_dim] (16-bit,
+ * strides in elements) by its token's position: the pair (a, b) becomes (a c - b s, b c + a s),
+ * where (a, b) are values (i, i + rotary_dim / 2), or (2i, 2i + 1) when `interleaved`. `inverse`
+ * rotates back, which is also the gradient with respect to x. The other values are copied. out has
+ * its own strides; out == x with x's strides works in place, any other overlap is undefined. A
+ * position outside [0, table_positions) sets *device_status (nullable) to 2 and leaves its token's
+ * rows of out as they were. rotary_dim is even, 2..head_dim, head_dim <= 1024, positions int32
+ * [token_count], tables fp32 [table_positions, rotary_dim / 2]. Arithmetic in fp32, one rounding. */
+int ar_rotary_positions(const void* x, int64_t x_token_stride, int64_t x_head_stride, void* out,
+                        int64_t out_token_stride, int64_t out_head_stride, const int32_t* positions, int token_count,
+                        int heads, int head_dim, int rotary_dim, int interleaved, int inverse, const float* cos_table,
+                        const float* sin_table, int table_positions, int* device_status, int dtype, void* stream);
+
+/* One layer's paged cache: k_pages and v_pages are 16-bit [page_count][kv_heads][page_size][head_dim],
+ * 16-byte aligned. page_size is a power of two, 16..1024; head_dim 64 or 128. */
+typedef struct {
+  void* k_pages;
+  void* v_pages;
+  int page_count;
+  int page_size;
+  int kv_heads;
+  int head_dim;
+  int dtype;
+} ar_paged_cache;
+
+/* The sequences of one call. Token rows [q_offsets[s], q_offsets[s + 1]) are sequence s's new tokens
+ * (none: an idle slot); kv_lengths[s] counts its cached tokens, the new ones included, so the new
+ * tokens' positions end at kv_lengths[s] - 1. Position p of sequence s lives in slot p % page_size
+ * of page page_table[s * page_table_stride + p / page_size]; entries no position needs are not read.
+ * Sequences may share pages that this call does not write. Device arrays: q_offsets int32
+ * [sequence_count + 1], kv_lengths int32 [sequence_count], page_table int32 [sequence_count,
+ * page_table_stride]. token_count is the number of rows in the call's buffers, max_query_tokens a
+ * bound on the new tokens of any sequence. A sequence with decreasing offsets, rows past token_count,
+ * more new tokens than max_query_tokens, or a length that is negative or beyond its page table's row
+ * sets *device_status (nullable) to 4 and is left out; a needed page id outside [0, page_count) sets
+ * it too (what is computed from that page is unspecified; nothing outside the arrays is touched).
+ * A status word keeps its first value until the caller clears it. */
+typedef struct {
+  int sequence_count;
+  int token_count;
+  int max_query_tokens;
+  int page_table_stride;
+  const int32_t* q_offsets;
+  const int32_t* kv_lengths;
+  const int32_t* page_table;
+} ar_paged_batch;
+
+/* Appends new tokens to the cache, rotation on the way. qkv: 16-bit rows of the fused projection,
+ * [token_count][(query_heads + 2 kv_heads) * head_dim] with row stride qkv_stride elements. Per
+ * token: bias (nullable, fp32 [(query_heads + 2 kv_heads) * head_dim]) is added, query and key heads
+ * are rotated at the token's position as ar_rotary_positions does, queries go to q_out (16-bit,
+ * [token_count][query_heads * head_dim], row stride q_out_stride; q_out == qkv with qkv_stride works
+ * in place; NULL or query_heads == 0: queries are left alone), keys and values to their page slots.
+ * fp32 arithmetic, one rounding. rotary_dim is a multiple of 16 up to head_dim, or 0 with NULL
+ * tables for no rotation. Strides are multiples of 8, qkv and q_out 16-byte aligned. A token whose
+ * position is negative (kv_lengths[s] below its new tokens) is left out; a position past
+ * table_positions sets *device_status to 2 and its token is left out. Rows no sequence owns are left
+ * out. Two tokens of one call must not share a page slot. */
+int ar_paged_append(const ar_paged_cache* cache, const ar_paged_batch* batch, const void* qkv, int64_t qkv_stride,
+                    const float* bias, int query_heads, void* q_out, int64_t q_out_stride, const float* cos_table,
+                    const float* sin_table, int table_positions, int rotary_dim, int interleaved, int* device_status,
+                    void* stream);
+
+/* Bytes of device workspace an ar_paged_attention call with these shapes needs (at most 64 MiB on a
+ * B200), or -1 for shapes it refuses. Independent of lengths and offsets. */
+int64_t ar_paged_attention_workspace(const ar_paged_cache* cache, const ar_paged_batch* batch, int query_heads);
+
+/* Attention of the new tokens over the cache, single tokens and chunks alike. For the token at
+ * position p of sequence s and query head h (KV head h / (query_heads / kv_heads)):
+ *   w_j = scale q_h . k_j over the cached positions j <= p (and j > p - sliding_window when that is
+ *   not 0);  out_h = sum_j softmax(w)_j v_j;  lse[token][h] = log2(sum_j 2^(w_j log2 e)).
+ * A row that sees no position (kv_lengths[s] below its new tokens) gets out 0 and lse -inf. Cached
+ * positions a row does not see, and slots past kv_lengths[s], do not touch it, whatever they hold.
+ * q: 16-bit, row stride q_stride elements, heads of a row contiguous; out: 16-bit, row stride
+ * out_stride, not overlapping q; both 16-byte aligned with strides multiples of 8. lse (nullable):
+ * fp32 [token_count][query_heads]. scale 0 means 1/sqrt(head_dim). query_heads / kv_heads <= 128.
+ * Scores, softmax statistics and sums are fp32; the probabilities are rounded to the 16-bit type for
+ * the product with v. Rows no sequence owns are left as they were. The same call on the same data
+ * gives the same bits. workspace: 16-byte aligned, its contents mean nothing between calls; calls
+ * whose work may overlap on the GPU (two streams, two captured graphs) each need their own. */
+int ar_paged_attention(const ar_paged_cache* cache, const ar_paged_batch* batch, const void* q, int64_t q_stride,
+                       int query_heads, float scale, int sliding_window, void* out, int64_t out_stride, float* lse,
+                       void* workspace, int64_t workspace_bytes, int* device_status, void* stream);
+
 /* Self-test of the library's bounded device waits. No counterpart in the reference: its kernels
  * never wait on one another. `ctas` CTAs (1..1024) wait on the grid barrier of the persistent
  * decode step for a counter value that nothing writes; the wait gives up after `spin_limit` polls
