@@ -1,13 +1,25 @@
 // Attention of new tokens over a paged KV cache (contract in include/attnrank_b200.h). For a row
 // (token at position p, query head h):
-//   out = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m),  x_j = scale log2(e) q . k_j,  m = max_j x_j,
+//   out = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m),  x_j = scale log2(e) q . k_j,
 //   lse = m + log2 sum_j 2^(x_j - m),
-// over the visible positions, in one pass with the running maximum and sum.
+// over the visible positions, in one pass with a running reference m and sum.
 //
-// One warp per row: lane l holds values l * D / 32 .. of q and of the accumulator, a score is a warp
-// sum, and positions the row does not see are never read.
+// Few rows a KV head (single tokens, a few drafted ones: at most 32 rows of new tokens x query heads
+// of the group): every K and V value is used once per call, so HBM bounds the kernel. K and V arrive
+// in 64-key blocks by TMA (192 KB of ring per SM, above the 45 KB that 6.5 TB/s x 1 us of latency
+// needs), and the products run on mma.sync m16n8k16 with the group's rows as its 16 rows: the 128 rows
+// of a tcgen05 tile would be 7/8 empty.
+//
+// Work: the batch's (sequence, KV head, key block) units form one line, cut into equal parts, one for
+// each CTA of one resident wave, wherever sequences begin or end; a part that holds a whole (sequence,
+// KV head) writes its rows, the others write fp32 partial sums that the second kernel joins in order.
+// Every CTA finds its part from q_offsets and kv_lengths itself, so no plan is made on the host and a
+// captured graph follows the lengths it finds.
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
+#include "async_copy.cuh"
 #include "common.cuh"
 #include "layer_kernels.h"
 #include "paged.h"
@@ -15,7 +27,631 @@
 namespace arb {
 namespace {
 
-constexpr int kThreads = 128;
+using namespace async;
+
+constexpr int kBlock = 64;          // keys a block
+constexpr int kCombineThreads = 256;
+constexpr float kRescaleThreshold = 8.0f;  // log2 units
+
+// One (sequence, KV head) of the line of work.
+struct FewTile {
+  int first_position;  // of the first new token; negative when fewer are cached than new
+  int first_key;       // smallest key any row sees (0 when none)
+  int block_begin;     // key blocks [block_begin, block_begin + blocks)
+  int blocks;          // at least 1
+};
+
+__device__ __forceinline__ FewTile few_tile(const PagedSequence& seq, int window) {
+  FewTile t;
+  t.first_position = seq.kv_len - seq.q_len;
+  t.first_key = window > 0 ? max(0, t.first_position - window + 1) : 0;
+  t.block_begin = t.first_key / kBlock;
+  t.blocks = max(1, (seq.kv_len + kBlock - 1) / kBlock - t.block_begin);
+  return t;
+}
+
+// Units of sequence s (0 without new tokens).
+__device__ __forceinline__ int64_t few_units(const PagedAttentionArgs& a, int s) {
+  const PagedSequence seq = paged_sequence(a.batch, s, a.status);
+  if (seq.q_len == 0) return 0;
+  return static_cast<int64_t>(few_tile(seq, a.sliding_window).blocks) * a.cache.kv_heads;
+}
+
+struct FewPlace {
+  int sequence;
+  int64_t before;  // units before the sequence
+};
+
+template <int kCount>
+struct PlanScratch {
+  int64_t sums[kCount / 32];
+  FewPlace place;
+};
+
+// Units of the whole batch; the block calls it.
+template <int kCount>
+__device__ __forceinline__ int64_t few_total(const PagedAttentionArgs& a, PlanScratch<kCount>& scratch) {
+  int64_t mine = 0;
+  for (int s = threadIdx.x; s < a.batch.sequences; s += kCount) mine += few_units(a, s);
+#pragma unroll
+  for (int offset = 16; offset > 0; offset >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, offset);
+  if ((threadIdx.x & 31) == 0) scratch.sums[threadIdx.x >> 5] = mine;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kCount / 32; ++w) total += scratch.sums[w];
+  __syncthreads();
+  return total;
+}
+
+// The sequence that holds unit `unit` (below the total); the block calls it.
+template <int kCount>
+__device__ __forceinline__ FewPlace few_locate(const PagedAttentionArgs& a, int64_t unit, PlanScratch<kCount>& scratch) {
+  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
+  int64_t before = 0;
+  for (int base = 0; base < a.batch.sequences; base += kCount) {
+    const int s = base + threadIdx.x;
+    const int64_t mine = s < a.batch.sequences ? few_units(a, s) : 0;
+    int64_t sum = mine;  // inclusive over the warp
+#pragma unroll
+    for (int offset = 1; offset < 32; offset <<= 1) {
+      const int64_t other = __shfl_up_sync(0xffffffffu, sum, offset);
+      if (lane >= offset) sum += other;
+    }
+    if (lane == 31) scratch.sums[warp] = sum;
+    __syncthreads();
+    int64_t all = before;
+#pragma unroll
+    for (int w = 0; w < kCount / 32; ++w) {
+      if (w == warp) sum += all;
+      all += scratch.sums[w];
+    }
+    if (unit >= sum - mine && unit < sum) scratch.place = {s, sum - mine};
+    __syncthreads();
+    if (unit < all) break;
+    before = all;
+  }
+  return scratch.place;
+}
+
+// Parts the line is cut into: one a CTA, each of at least one unit.
+__device__ __forceinline__ int few_parts(int64_t total, int ctas) {
+  return static_cast<int>(min(total, static_cast<int64_t>(ctas)));
+}
+// Where part c of `parts` begins, and the part that holds a unit.
+__device__ __forceinline__ int64_t part_begin(int64_t total, int c, int parts) { return total * c / parts; }
+__device__ __forceinline__ int part_of(int64_t total, int64_t unit, int parts) {
+  return static_cast<int>(((unit + 1) * parts - 1) / total);
+}
+
+// Partial sums of a tile that several CTAs share. A CTA has two slots: 1 for a tile that begins in its
+// part, 0 for one that began before it.
+template <int kRows, int kDim>
+struct FewPartials {
+  float* sums;    // [2 ctas][kRows][kDim]
+  float2* stats;  // [2 ctas][kRows]: reference and sum
+  __device__ __forceinline__ FewPartials(void* workspace, int ctas)
+      : sums(static_cast<float*>(workspace)),
+        stats(reinterpret_cast<float2*>(sums + static_cast<int64_t>(2) * ctas * kRows * kDim)) {}
+};
+
+constexpr int64_t few_workspace(int rows, int dim, int ctas) {
+  return static_cast<int64_t>(2) * ctas * rows * (dim * sizeof(float) + sizeof(float2));
+}
+
+// A CTA has kGroups groups of four warps, a group for each 16 rows; they read the same blocks. One
+// group: two CTAs an SM with three stages each; two: one CTA with six (its 128 accumulators a thread
+// and the query operands of 32 rows would not fit four warps' registers).
+template <int kGroups, int kDim>
+struct FewShared {
+  static constexpr int kThreads = (4 * kGroups + 1) * 32;
+  static constexpr int kCtasPerSm = kGroups == 1 ? 2 : 1;
+  static constexpr int kStages = kGroups == 1 ? 3 : 6;
+  static constexpr int kRows = 16 * kGroups;
+  static constexpr uint32_t kBlockBytes = kBlock * kDim * 2;  // of K, or of V
+  static constexpr int kPad = 36;                             // floats a merge row of 32 takes
+  uint64_t full[kStages];
+  uint64_t empty[kStages];
+  volatile int abort;
+  int poison[kGroups][2];  // of this segment and the next, in turn
+  PlanScratch<kThreads> plan;
+  float2 stats[kGroups][4][16];
+  alignas(16) float merge[kGroups][4][16][kPad];
+  static constexpr size_t bytes() { return 2 * kStages * kBlockBytes + sizeof(FewShared) + 1024; }
+};
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t address, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(address));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t address, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(address));
+}
+
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same_v<T, __half>) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+
+__device__ __forceinline__ void group_barrier(int group) {
+  if (group == 0) {
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+  } else {
+    asm volatile("bar.sync 2, 128;" ::: "memory");
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ bool nonfinite_half(uint32_t bits) {
+  constexpr uint32_t kExponent = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
+  return (bits & kExponent) == kExponent;
+}
+
+// Two V values of keys `key` and `key + 1` of a block that not every row sees whole. A probability of
+// zero times a NaN or infinity is NaN, so values outside [first, end) (slots nobody wrote, keys no row
+// sees) become 0, and so does a value that is not finite, which `poison` reports: the rows that see
+// it get it added at the end.
+template <typename T>
+__device__ __forceinline__ uint32_t clean_pair(uint32_t pair, int key, int first, int end, bool& poison) {
+  const bool in0 = key >= first && key < end;
+  const bool in1 = key + 1 >= first && key + 1 < end;
+  const bool bad0 = nonfinite_half<T>(pair);
+  const bool bad1 = nonfinite_half<T>(pair >> 16);
+  poison |= (in0 && bad0) || (in1 && bad1);
+  return (in0 && !bad0 ? pair & 0xffffu : 0u) | (in1 && !bad1 ? pair & 0xffff0000u : 0u);
+}
+
+// Sum of the values of column `column` that are not finite, over the keys [first, last] of sequence s.
+template <typename T, int kDim>
+__device__ float nonfinite_sum(const PagedAttentionArgs& a, int s, int kv_head, int first, int last, int column) {
+  float sum = 0.0f;
+  for (int key = first; key <= last; ++key) {
+    const int page = paged_page(a.cache, a.batch, s, key >> a.cache.page_shift, a.status);
+    const int64_t row = ((static_cast<int64_t>(page) * a.cache.kv_heads + kv_head) << a.cache.page_shift) +
+                        (key & ((1 << a.cache.page_shift) - 1));
+    const float v = static_cast<float>(static_cast<const T*>(a.cache.v_pages)[row * kDim + column]);
+    if (!isfinite(v)) sum += v;
+  }
+  return sum;
+}
+
+template <typename T, int kGroups, int kDim>
+__global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<kGroups, kDim>::kCtasPerSm)
+    paged_attention_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                               const PagedAttentionArgs a) {
+  using Shared = FewShared<kGroups, kDim>;
+  constexpr int kThreads = Shared::kThreads;
+  constexpr int kStages = Shared::kStages;
+  constexpr int kRows = Shared::kRows;
+  constexpr uint32_t kBlockBytes = Shared::kBlockBytes;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Shared& sh = *reinterpret_cast<Shared*>(smem + 2 * kStages * kBlockBytes);
+  const uint32_t k_smem = smem_u32(smem);
+  const uint32_t v_smem = k_smem + kStages * kBlockBytes;
+  const int tid = threadIdx.x;
+  const int warp = tid >> 5;
+  const int lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(smem_u32(&sh.full[i]), 1);
+      mbar_init(smem_u32(&sh.empty[i]), 4 * kGroups);
+    }
+    sh.abort = 0;
+    for (int i = 0; i < kGroups; ++i) sh.poison[i][0] = sh.poison[i][1] = 0;
+    mbar_init_fence();
+    prefetch_map(&k_map);
+    prefetch_map(&v_map);
+  }
+  const int64_t total = few_total<kThreads>(a, sh.plan);  // its barriers cover the set-up above
+  const int parts = few_parts(total, gridDim.x);
+  release_dependents();  // the joining kernel waits for this one's completion by itself
+  if (blockIdx.x >= parts) return;
+  const int64_t begin = part_begin(total, blockIdx.x, parts);
+  const int64_t end = part_begin(total, blockIdx.x + 1, parts);
+  const FewPlace place = few_locate<kThreads>(a, begin, sh.plan);
+
+  // walk of the part, the same for every role: segments of one (sequence, KV head)
+  int s = place.sequence;
+  PagedSequence seq = paged_sequence(a.batch, s, nullptr);
+  FewTile tile = few_tile(seq, a.sliding_window);
+  int kv_head = static_cast<int>((begin - place.before) / tile.blocks);
+  int block = static_cast<int>(begin - place.before - static_cast<int64_t>(kv_head) * tile.blocks);
+  int64_t left = end - begin;
+  auto next_tile = [&] {
+    block = 0;
+    if (++kv_head < a.cache.kv_heads) return;
+    kv_head = 0;
+    do {  // `left` units remain, so a sequence with new tokens follows
+      seq = paged_sequence(a.batch, ++s, nullptr);
+    } while (seq.q_len == 0 && s + 1 < a.batch.sequences);
+    tile = few_tile(seq, a.sliding_window);
+  };
+
+  const int page_rows = min(1 << a.cache.page_shift, kBlock);  // rows of one TMA box
+  const int boxes = kBlock / page_rows;
+  uint32_t turn = 0;  // blocks done so far: stage turn % kStages, phase turn / kStages
+
+  if (warp == 4 * kGroups) {
+    // ---------------------------------------------------------------------------------- producer
+    bool ok = true;
+    while (ok && left > 0) {
+      const int count = static_cast<int>(min(left, static_cast<int64_t>(tile.blocks - block)));
+      auto page_at = [&](int b) {  // this lane's page of block b, -1 when no row needs it
+        const int key = (tile.block_begin + b) * kBlock + lane * page_rows;
+        if (lane >= boxes || key >= seq.kv_len || key + page_rows <= tile.first_key) return -1;
+        return paged_page(a.cache, a.batch, s, key >> a.cache.page_shift, a.status);
+      };
+      int page = page_at(block);
+      for (int i = 0; i < count; ++i, ++turn) {
+        const int following = i + 1 < count ? page_at(block + i + 1) : -1;  // its latency hides behind the wait
+        const int stage = turn % kStages;
+        const uint32_t round = turn / kStages;
+        if (round > 0 && !mbar_wait(smem_u32(&sh.empty[stage]), (round - 1) & 1, &sh.abort)) {
+          ok = false;
+          break;
+        }
+        const uint32_t bar = smem_u32(&sh.full[stage]);
+        const uint32_t loads = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        if (lane == 0) mbar_expect_tx(bar, loads * page_rows * kDim * 2 * 2);
+        __syncwarp();
+        if (page >= 0) {
+          const int key = (tile.block_begin + block + i) * kBlock + lane * page_rows;
+          const int row = ((page * a.cache.kv_heads + kv_head) << a.cache.page_shift) +
+                          (key & ((1 << a.cache.page_shift) - 1));
+          const uint32_t to = stage * kBlockBytes + lane * page_rows * kDim * 2;
+          tma_load_3d(k_smem + to, &k_map, 0, row, 0, bar);
+          tma_load_3d(v_smem + to, &v_map, 0, row, 0, bar);
+        }
+        page = following;
+      }
+      left -= count;
+      if (left > 0) next_tile();
+    }
+    if (!ok) {  // a consumer gave up: the loads in flight land before the shared memory is released
+      if (lane == 0) {
+        report_status(a.status, kStatusWaitTimeout);
+        sh.abort = 1;
+      }
+      for (uint32_t t = turn > kStages ? turn - kStages : 0; t < turn; ++t) {
+        mbar_wait(smem_u32(&sh.full[t % kStages]), (t / kStages) & 1, nullptr);
+      }
+    }
+    return;
+  }
+
+  // ------------------------------------------------------------------------------------ consumers
+  const int group = a.query_heads / a.cache.kv_heads;
+  const int part16 = warp >> 2;  // the warp's group of 16 rows
+  const int quarter = warp & 3;  // its 16 keys of a block
+  const int g = lane >> 2;
+  const int t4 = lane & 3;
+  // this lane's addresses inside a block: [page][64-wide half][row][128 bytes], 16-byte chunks XORed
+  // with the row's low bits (the TMA's 128-byte swizzle)
+  auto row_offset = [&](int key) {
+    const int page = key / page_rows;
+    const int row = key - page * page_rows;
+    return static_cast<uint32_t>(page * page_rows * kDim * 2 + row * 128);
+  };
+  const int half_bytes = page_rows * 128;
+  const uint32_t k_row = row_offset(quarter * 16 + (lane >> 4) * 8 + (lane & 7));
+  const int k_chunk = (lane >> 3) & 1;
+  const uint32_t v_row = row_offset(quarter * 16 + ((lane >> 3) & 1) * 8 + (lane & 7));
+  const int v_chunk = lane >> 4;
+  const uint32_t swizzle = lane & 7;  // both rows are 8i + (lane & 7)
+  auto chunk_offset = [&](int chunk) {  // 16-byte chunk 0..kDim/8-1 of the lane's row
+    return static_cast<uint32_t>((chunk >> 3) * half_bytes + (((chunk & 7) ^ swizzle) << 4));
+  };
+  bool ok = true;
+  int segment = 0;
+  while (ok && left > 0) {
+    const int count = static_cast<int>(min(left, static_cast<int64_t>(tile.blocks - block)));
+    const int rows = seq.q_len * group;
+    // Q as MMA operands: the lane holds rows g and g + 8 of its group's 16
+    uint32_t q[kDim / 16][4];
+    int last_key[2];   // largest key each of the lane's rows sees, below 0: none
+    int first_key[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int row = part16 * 16 + e * 8 + g;
+      const int token = row / group;
+      const bool in = row < rows;
+      last_key[e] = in ? tile.first_position + token : -1;
+      first_key[e] = a.sliding_window > 0 ? max(0, tile.first_position + token - a.sliding_window + 1) : 0;
+      const T* from = static_cast<const T*>(a.q) + (seq.q_begin + (in ? token : 0)) * a.q_stride +
+                      (kv_head * group + (in ? row - token * group : 0)) * kDim + 2 * t4;
+#pragma unroll
+      for (int k = 0; k < kDim / 16; ++k) {
+        q[k][e] = in ? __ldg(reinterpret_cast<const uint32_t*>(from + 16 * k)) : 0u;
+        q[k][2 + e] = in ? __ldg(reinterpret_cast<const uint32_t*>(from + 16 * k + 8)) : 0u;
+      }
+    }
+    float o[kDim / 8][4];
+#pragma unroll
+    for (int d = 0; d < kDim / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
+    float reference[2] = {-INFINITY, -INFINITY};
+    float l[2] = {0.0f, 0.0f};
+    bool poison = false;
+    for (int i = 0; i < count; ++i, ++turn) {
+      const int stage = turn % kStages;
+      const bool ready = mbar_wait(smem_u32(&sh.full[stage]), (turn / kStages) & 1, &sh.abort);
+      if (!__all_sync(0xffffffffu, ready)) {
+        ok = false;
+        break;
+      }
+      const int key0 = (tile.block_begin + block + i) * kBlock;
+      // does every row see every key of the block?
+      const bool whole = key0 + kBlock - 1 <= tile.first_position &&
+                         (a.sliding_window == 0 || key0 >= seq.kv_len - a.sliding_window);
+      const uint32_t k_at = k_smem + stage * kBlockBytes + k_row;
+      const uint32_t v_at = v_smem + stage * kBlockBytes + v_row;
+      float x[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kDim / 16; ++k) {
+        uint32_t b[4];
+        ldmatrix_x4(k_at + chunk_offset(2 * k + k_chunk), b);
+        mma_16816<T>(x[0], q[k], b[0], b[1]);
+        mma_16816<T>(x[1], q[k], b[2], b[3]);
+      }
+      const int key = key0 + quarter * 16 + 2 * t4;  // of x[0][0]
+      uint32_t p[4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {  // rows g, g + 8
+        float top = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float& v = x[n][2 * e + c];
+            const int at = key + 8 * n + c;
+            v = whole || (at <= last_key[e] && at >= first_key[e]) ? v * a.scale_log2 : -INFINITY;
+            top = fmaxf(top, v);
+          }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // the reference moves only when the block's maximum exceeds it by more than the threshold, so
+        // probabilities stay below 2^8 and the sums are rarely rescaled
+        const bool move = top > reference[e] + kRescaleThreshold || (reference[e] == -INFINITY && top != -INFINITY);
+        if (__any_sync(0xffffffffu, move)) {
+          const float factor = move ? (reference[e] == -INFINITY ? 0.0f : ex2_ftz(reference[e] - top)) : 1.0f;
+          if (move) reference[e] = top;
+          l[e] *= factor;
+#pragma unroll
+          for (int d = 0; d < kDim / 8; ++d) {
+            o[d][2 * e] *= factor;
+            o[d][2 * e + 1] *= factor;
+          }
+        }
+        const float base = reference[e] == -INFINITY ? 0.0f : reference[e];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float p0 = ex2_ftz(x[n][2 * e] - base);
+          const float p1 = ex2_ftz(x[n][2 * e + 1] - base);
+          l[e] += p0 + p1;
+          p[2 * n + e] = pack2<T>(p0, p1);
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < kDim / 16; ++d) {
+        uint32_t b[4];
+        ldmatrix_x4_trans(v_at + chunk_offset(2 * d + v_chunk), b);
+        if (!whole) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            b[r] = clean_pair<T>(b[r], key + 8 * (r & 1), tile.first_key, seq.kv_len, poison);
+          }
+        }
+        mma_16816<T>(o[2 * d], p, b[0], b[1]);
+        mma_16816<T>(o[2 * d + 1], p, b[2], b[3]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.empty[stage]));
+    }
+    if (!ok) break;
+
+    // ---- join the four warps' sums: common reference, then 32 columns at a time through shared memory
+    if (__any_sync(0xffffffffu, poison) && lane == 0) sh.poison[part16][segment & 1] = 1;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+      if (t4 == 0) sh.stats[part16][quarter][e * 8 + g] = make_float2(reference[e], l[e]);
+    }
+    group_barrier(part16);
+    const bool poisoned = sh.poison[part16][segment & 1] != 0;
+    // the other flag's readers have passed the last segment's barriers
+    if (quarter == 0 && lane == 0) sh.poison[part16][(segment + 1) & 1] = 0;
+    const bool begins = block == 0;
+    const bool complete = begins && count == tile.blocks;
+    const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (begins ? 1 : 0);
+    const FewPartials<kRows, kDim> partials(a.workspace, gridDim.x);
+    auto joined = [&](int row) {  // (reference, sum) of one of the 16 rows over the warps
+      float2 all = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) all.x = fmaxf(all.x, sh.stats[part16][w][row].x);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float2 part = sh.stats[part16][w][row];
+        all.y += part.y * (part.x == -INFINITY ? 0.0f : ex2_ftz(part.x - all.x));
+      }
+      return all;
+    };
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float factor = reference[e] == -INFINITY ? 0.0f : ex2_ftz(reference[e] - joined(e * 8 + g).x);
+#pragma unroll
+      for (int d = 0; d < kDim / 8; ++d) {
+        o[d][2 * e] *= factor;
+        o[d][2 * e + 1] *= factor;
+      }
+    }
+    // this thread's place in a pass: 16 rows x 32 columns, four columns a thread
+    const int merge_row = quarter * 4 + (lane >> 3);
+    const int row = part16 * 16 + merge_row;
+    const int token = row / group;
+    const int head = kv_head * group + row - token * group;
+    const float2 all = joined(merge_row);
+    const float inverse = all.y != 0.0f ? 1.0f / all.y : 0.0f;
+#pragma unroll
+    for (int c = 0; c < kDim / 32; ++c) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          *reinterpret_cast<float2*>(&sh.merge[part16][quarter][e * 8 + g][d * 8 + 2 * t4]) =
+              make_float2(o[4 * c + d][2 * e], o[4 * c + d][2 * e + 1]);
+        }
+      }
+      group_barrier(part16);
+      if (row < rows) {
+        const int column = c * 32 + (lane & 7) * 4;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float4 part = *reinterpret_cast<const float4*>(&sh.merge[part16][w][merge_row][(lane & 7) * 4]);
+          sum.x += part.x;
+          sum.y += part.y;
+          sum.z += part.z;
+          sum.w += part.w;
+        }
+        if (poisoned) {
+          const int position = tile.first_position + token;
+          const int low = max((tile.block_begin + block) * kBlock,
+                              a.sliding_window > 0 ? position - a.sliding_window + 1 : 0);
+          const int high = min((tile.block_begin + block + count) * kBlock - 1, position);
+          sum.x += nonfinite_sum<T, kDim>(a, s, kv_head, low, high, column);
+          sum.y += nonfinite_sum<T, kDim>(a, s, kv_head, low, high, column + 1);
+          sum.z += nonfinite_sum<T, kDim>(a, s, kv_head, low, high, column + 2);
+          sum.w += nonfinite_sum<T, kDim>(a, s, kv_head, low, high, column + 3);
+        }
+        if (complete) {
+          T* to = static_cast<T*>(a.out) + (seq.q_begin + token) * a.out_stride + head * kDim + column;
+          *reinterpret_cast<uint2*>(to) =
+              make_uint2(pack2<T>(sum.x * inverse, sum.y * inverse), pack2<T>(sum.z * inverse, sum.w * inverse));
+          if (column == 0 && a.lse != nullptr) {
+            a.lse[static_cast<int64_t>(seq.q_begin + token) * a.query_heads + head] =
+                all.y != 0.0f ? all.x + log2f(all.y) : -INFINITY;
+          }
+        } else {
+          *reinterpret_cast<float4*>(partials.sums + (slot * kRows + row) * kDim + column) = sum;
+          if (column == 0) partials.stats[slot * kRows + row] = all;
+        }
+      }
+      group_barrier(part16);
+    }
+    ++segment;
+    left -= count;
+    if (left > 0) next_tile();
+  }
+  if (!ok && lane == 0) {
+    report_status(a.status, kStatusWaitTimeout);
+    sh.abort = 1;
+  }
+}
+
+// Joins the parts of the tile that the boundary between CTAs c and c + 1 cuts, for the first such
+// boundary of each tile, in the order of the CTAs.
+template <typename T, int kRows, int kDim>
+__global__ void __launch_bounds__(kCombineThreads) paged_attention_few_join_kernel(const PagedAttentionArgs a, int ctas) {
+  __shared__ PlanScratch<kCombineThreads> plan;
+  const int64_t total = few_total<kCombineThreads>(a, plan);
+  const int parts = few_parts(total, ctas);
+  const int c = blockIdx.x;  // the boundary between parts c and c + 1
+  const int64_t at = part_begin(total, c + 1, max(parts, 1));
+  bool cut = c + 1 < parts;
+  PagedSequence seq{};
+  FewTile tile{};
+  int kv_head = 0;
+  int last = 0;  // part that holds the tile's last unit
+  if (cut) {
+    const FewPlace place = few_locate<kCombineThreads>(a, at, plan);
+    seq = paged_sequence(a.batch, place.sequence, nullptr);
+    tile = few_tile(seq, a.sliding_window);
+    kv_head = static_cast<int>((at - place.before) / tile.blocks);
+    const int64_t tile_begin = place.before + static_cast<int64_t>(kv_head) * tile.blocks;
+    cut = tile_begin < at && part_begin(total, c, parts) <= tile_begin;
+    last = part_of(total, tile_begin + tile.blocks - 1, parts);
+  }
+  // every CTA waits, so that this grid does not complete before the one whose sums it reads
+  wait_for_producer();
+  if (!cut) return;
+  const int group = a.query_heads / a.cache.kv_heads;
+  const int rows = seq.q_len * group;
+  const FewPartials<kRows, kDim> partials(a.workspace, ctas);
+  constexpr int kBatch = 8;  // parts whose loads are in flight together
+  for (int item = threadIdx.x; item < rows * (kDim / 4); item += kCombineThreads) {
+    const int row = item / (kDim / 4);
+    const int column = (item - row * (kDim / 4)) * 4;
+    float top = -INFINITY;
+    float sum = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int first = c; first <= last; first += kBatch) {
+      float2 stats[kBatch];
+      float4 piece[kBatch];
+      float high = top;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int part = first + i;
+        stats[i] = make_float2(-INFINITY, 0.0f);
+        piece[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (part <= last) {
+          const int64_t at_row = (static_cast<int64_t>(part) * 2 + (part == c ? 1 : 0)) * kRows + row;
+          stats[i] = partials.stats[at_row];
+          piece[i] = *reinterpret_cast<const float4*>(partials.sums + at_row * kDim + column);
+        }
+        high = fmaxf(high, stats[i].x);
+      }
+      const float keep = top == -INFINITY ? 0.0f : ex2_ftz(top - high);
+      sum *= keep;
+      o.x *= keep;
+      o.y *= keep;
+      o.z *= keep;
+      o.w *= keep;
+      top = high;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const float factor = stats[i].x == -INFINITY ? 0.0f : ex2_ftz(stats[i].x - top);
+        sum += factor * stats[i].y;
+        o.x += factor * piece[i].x;
+        o.y += factor * piece[i].y;
+        o.z += factor * piece[i].z;
+        o.w += factor * piece[i].w;
+      }
+    }
+    const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
+    const int token = row / group;
+    const int head = kv_head * group + row - token * group;
+    T* to = static_cast<T*>(a.out) + (seq.q_begin + token) * a.out_stride + head * kDim + column;
+    *reinterpret_cast<uint2*>(to) =
+        make_uint2(pack2<T>(o.x * inverse, o.y * inverse), pack2<T>(o.z * inverse, o.w * inverse));
+    if (column == 0 && a.lse != nullptr) {
+      a.lse[static_cast<int64_t>(seq.q_begin + token) * a.query_heads + head] =
+          sum != 0.0f ? top + log2f(sum) : -INFINITY;
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------- many rows
+constexpr int kRowsThreads = 128;
 
 template <typename T, int kDim>
 __device__ __forceinline__ void load_lane(const T* row, float (&v)[kDim / 32]) {
@@ -29,9 +665,11 @@ __device__ __forceinline__ void load_lane(const T* row, float (&v)[kDim / 32]) {
   }
 }
 
+// One warp per row: lane l holds values l * D / 32 .. of q and of the accumulator, a score is a warp
+// sum, and positions the row does not see are never read.
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kThreads) paged_attention_rows_kernel(const PagedAttentionArgs a) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(kRowsThreads) paged_attention_rows_kernel(const PagedAttentionArgs a) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kRowsThreads / 32) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const int token = static_cast<int>(row / a.query_heads);
   const int head = static_cast<int>(row - static_cast<int64_t>(token) * a.query_heads);
@@ -86,22 +724,93 @@ __global__ void __launch_bounds__(kThreads) paged_attention_rows_kernel(const Pa
   }
 }
 
+// ------------------------------------------------------------------------------------- launches
+// [rows of the pool][kDim] as boxes of 64 columns x `rows` rows x (kDim / 64) halves
+template <typename T>
+bool encode_pages(CUtensorMap* map, const PagedCache& c, void* pages, int rows) {
+  PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
+  if (encode == nullptr) return false;
+  const cuuint64_t pool_rows = (static_cast<cuuint64_t>(c.page_count) * c.kv_heads) << c.page_shift;
+  const cuuint64_t dims[3] = {64, pool_rows, static_cast<cuuint64_t>(c.head_dim / 64)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(c.head_dim) * 2, 128};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(rows), static_cast<cuuint32_t>(c.head_dim / 64)};
+  const cuuint32_t element_strides[3] = {1, 1, 1};
+  const CUtensorMapDataType type =
+      std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return encode(map, type, 3, pages, dims, strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int kGroups>
+int few_ctas() {
+  return sm_count() * FewShared<kGroups, 128>::kCtasPerSm;
+}
+
+template <typename T, int kGroups, int kDim>
+cudaError_t launch_few(const PagedAttentionArgs& a, cudaStream_t stream) {
+  using Shared = FewShared<kGroups, kDim>;
+  static_assert(Shared::kCtasPerSm * (Shared::bytes() + 1024) <= 228 * 1024, "the CTAs of an SM share its shared memory");
+  int device = 0;
+  cudaGetDevice(&device);
+  static uint64_t configured = 0;  // the shared-memory opt-in is a per-device attribute
+  if (device >= 64 || !(configured & (1ull << device))) {
+    const cudaError_t status =
+        cudaFuncSetAttribute(paged_attention_few_kernel<T, kGroups, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(Shared::bytes()));
+    if (status != cudaSuccess) return status;
+    if (device < 64) configured |= 1ull << device;
+  }
+  CUtensorMap k_map, v_map;
+  const int rows = std::min(1 << a.cache.page_shift, kBlock);
+  if (!encode_pages<T>(&k_map, a.cache, a.cache.k_pages, rows) ||
+      !encode_pages<T>(&v_map, a.cache, a.cache.v_pages, rows)) {
+    return cudaErrorInvalidValue;
+  }
+  const int ctas = few_ctas<kGroups>();
+  paged_attention_few_kernel<T, kGroups, kDim><<<ctas, Shared::kThreads, Shared::bytes(), stream>>>(k_map, v_map, a);
+  cudaError_t status = cudaGetLastError();
+  if (status != cudaSuccess) return status;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(ctas - 1);
+  config.blockDim = dim3(kCombineThreads);
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  status = cudaLaunchKernelEx(&config, paged_attention_few_join_kernel<T, Shared::kRows, kDim>, a, ctas);
+  return status != cudaSuccess ? status : cudaGetLastError();
+}
+
+template <typename T, int kDim>
+cudaError_t launch_dim(const PagedAttentionArgs& a, cudaStream_t stream) {
+  const int64_t rows = static_cast<int64_t>(a.batch.max_query) * (a.query_heads / a.cache.kv_heads);
+  if (rows <= 16) return launch_few<T, 1, kDim>(a, stream);
+  if (rows <= 32) return launch_few<T, 2, kDim>(a, stream);
+  const int64_t all = static_cast<int64_t>(a.batch.tokens) * a.query_heads;
+  paged_attention_rows_kernel<T, kDim>
+      <<<static_cast<unsigned>((all + kRowsThreads / 32 - 1) / (kRowsThreads / 32)), kRowsThreads, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
 }  // namespace
 
-int64_t paged_attention_workspace(const PagedCache&, const PagedBatch&, int) { return 0; }
+int64_t paged_attention_workspace(const PagedCache& cache, const PagedBatch& batch, int query_heads) {
+  const int64_t rows = static_cast<int64_t>(batch.max_query) * (query_heads / cache.kv_heads);
+  if (rows <= 16) return few_workspace(16, cache.head_dim, few_ctas<1>());
+  if (rows <= 32) return few_workspace(32, cache.head_dim, few_ctas<2>());
+  return 0;
+}
 
 cudaError_t launch_paged_attention(const PagedAttentionArgs& a, cudaStream_t stream) {
   if (a.batch.tokens <= 0 || a.batch.sequences <= 0) return cudaSuccess;
-  const int64_t rows = static_cast<int64_t>(a.batch.tokens) * a.query_heads;
-  const int64_t grid = (rows + kThreads / 32 - 1) / (kThreads / 32);
-  auto run = [&](auto kernel) { kernel<<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(a); };
   if (a.cache.dtype == kActFp16) {
-    a.cache.head_dim == 128 ? run(paged_attention_rows_kernel<__half, 128>) : run(paged_attention_rows_kernel<__half, 64>);
-  } else {
-    a.cache.head_dim == 128 ? run(paged_attention_rows_kernel<__nv_bfloat16, 128>)
-                            : run(paged_attention_rows_kernel<__nv_bfloat16, 64>);
+    return a.cache.head_dim == 128 ? launch_dim<__half, 128>(a, stream) : launch_dim<__half, 64>(a, stream);
   }
-  return cudaGetLastError();
+  return a.cache.head_dim == 128 ? launch_dim<__nv_bfloat16, 128>(a, stream)
+                                 : launch_dim<__nv_bfloat16, 64>(a, stream);
 }
 
 }  // namespace arb
