@@ -290,6 +290,7 @@ int ar_paged_attention(const ar_paged_cache* cache, const ar_paged_batch* batch,
     args.cache = checked_cache(who, cache);
     args.batch = checked_batch(who, batch, args.cache);
     check_query_heads(who, query_heads, args.cache);
+    require(args.batch.max_query <= 1 << 24, who, "max_query_tokens must be at most 2^24");
     const int64_t width = static_cast<int64_t>(query_heads) * args.cache.head_dim;
     require(q_stride >= width && q_stride % 8 == 0 && out_stride >= width && out_stride % 8 == 0, who,
             "q_stride and out_stride must be multiples of 8 and hold the query heads");

@@ -1,5 +1,6 @@
 // Serving operators: launchers of the scaled rotary table and rotation (rotary.cu), the append to a
-// paged KV cache (paged_append.cu) and the attention over it (paged_attention.cu). All pointers are
+// paged KV cache (paged_append.cu) and the attention over it
+// (paged_attention.cu, paged_attention_tc.cu). All pointers are
 // device pointers; all launches are asynchronous on `stream`. The contracts are those of
 // include/attnrank_b200.h; argument checks are in capi_paged.cu.
 #pragma once
@@ -99,6 +100,9 @@ struct PagedAttentionArgs {
 };
 int64_t paged_attention_workspace(const PagedCache& cache, const PagedBatch& batch, int query_heads);
 cudaError_t launch_paged_attention(const PagedAttentionArgs& args, cudaStream_t stream);
+// The form for more than a few rows a KV head (paged_attention_tc.cu).
+int64_t paged_attention_chunk_workspace(int head_dim);
+cudaError_t launch_paged_attention_chunk(const PagedAttentionArgs& args, cudaStream_t stream);
 
 // ------------------------------------------------------------------------------ device helpers
 #ifdef __CUDACC__

@@ -11,10 +11,11 @@
 // of a tcgen05 tile would be 7/8 empty.
 //
 // Work: the batch's (sequence, KV head, key block) units form one line, cut into equal parts, one for
-// each CTA of one resident wave, wherever sequences begin or end; a part that holds a whole (sequence,
-// KV head) writes its rows, the others write fp32 partial sums that the second kernel joins in order.
-// Every CTA finds its part from q_offsets and kv_lengths itself, so no plan is made on the host and a
-// captured graph follows the lengths it finds.
+// each CTA of one resident wave (paged_plan.cuh); a part that holds a whole (sequence, KV head) writes
+// its rows, the others write fp32 partial sums that the second kernel joins in order. Every CTA finds
+// its part from q_offsets and kv_lengths itself, so no plan is made on the host and a captured graph
+// follows the lengths it finds.
+// More rows: paged_attention_tc.cu.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -23,6 +24,7 @@
 #include "common.cuh"
 #include "layer_kernels.h"
 #include "paged.h"
+#include "paged_plan.cuh"
 
 namespace arb {
 namespace {
@@ -55,89 +57,6 @@ __device__ __forceinline__ int64_t few_units(const PagedAttentionArgs& a, int s)
   const PagedSequence seq = paged_sequence(a.batch, s, a.status);
   if (seq.q_len == 0) return 0;
   return static_cast<int64_t>(few_tile(seq, a.sliding_window).blocks) * a.cache.kv_heads;
-}
-
-struct FewPlace {
-  int sequence;
-  int64_t before;  // units before the sequence
-};
-
-template <int kCount>
-struct PlanScratch {
-  int64_t sums[kCount / 32];
-  FewPlace place;
-};
-
-// Units of the whole batch; the block calls it.
-template <int kCount>
-__device__ __forceinline__ int64_t few_total(const PagedAttentionArgs& a, PlanScratch<kCount>& scratch) {
-  int64_t mine = 0;
-  for (int s = threadIdx.x; s < a.batch.sequences; s += kCount) mine += few_units(a, s);
-#pragma unroll
-  for (int offset = 16; offset > 0; offset >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, offset);
-  if ((threadIdx.x & 31) == 0) scratch.sums[threadIdx.x >> 5] = mine;
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < kCount / 32; ++w) total += scratch.sums[w];
-  __syncthreads();
-  return total;
-}
-
-// The sequence that holds unit `unit` (below the total); the block calls it.
-template <int kCount>
-__device__ __forceinline__ FewPlace few_locate(const PagedAttentionArgs& a, int64_t unit, PlanScratch<kCount>& scratch) {
-  const int lane = threadIdx.x & 31;
-  const int warp = threadIdx.x >> 5;
-  int64_t before = 0;
-  for (int base = 0; base < a.batch.sequences; base += kCount) {
-    const int s = base + threadIdx.x;
-    const int64_t mine = s < a.batch.sequences ? few_units(a, s) : 0;
-    int64_t sum = mine;  // inclusive over the warp
-#pragma unroll
-    for (int offset = 1; offset < 32; offset <<= 1) {
-      const int64_t other = __shfl_up_sync(0xffffffffu, sum, offset);
-      if (lane >= offset) sum += other;
-    }
-    if (lane == 31) scratch.sums[warp] = sum;
-    __syncthreads();
-    int64_t all = before;
-#pragma unroll
-    for (int w = 0; w < kCount / 32; ++w) {
-      if (w == warp) sum += all;
-      all += scratch.sums[w];
-    }
-    if (unit >= sum - mine && unit < sum) scratch.place = {s, sum - mine};
-    __syncthreads();
-    if (unit < all) break;
-    before = all;
-  }
-  return scratch.place;
-}
-
-// Parts the line is cut into: one a CTA, each of at least one unit.
-__device__ __forceinline__ int few_parts(int64_t total, int ctas) {
-  return static_cast<int>(min(total, static_cast<int64_t>(ctas)));
-}
-// Where part c of `parts` begins, and the part that holds a unit.
-__device__ __forceinline__ int64_t part_begin(int64_t total, int c, int parts) { return total * c / parts; }
-__device__ __forceinline__ int part_of(int64_t total, int64_t unit, int parts) {
-  return static_cast<int>(((unit + 1) * parts - 1) / total);
-}
-
-// Partial sums of a tile that several CTAs share. A CTA has two slots: 1 for a tile that begins in its
-// part, 0 for one that began before it.
-template <int kRows, int kDim>
-struct FewPartials {
-  float* sums;    // [2 ctas][kRows][kDim]
-  float2* stats;  // [2 ctas][kRows]: reference and sum
-  __device__ __forceinline__ FewPartials(void* workspace, int ctas)
-      : sums(static_cast<float*>(workspace)),
-        stats(reinterpret_cast<float2*>(sums + static_cast<int64_t>(2) * ctas * kRows * kDim)) {}
-};
-
-constexpr int64_t few_workspace(int rows, int dim, int ctas) {
-  return static_cast<int64_t>(2) * ctas * rows * (dim * sizeof(float) + sizeof(float2));
 }
 
 // A CTA has kGroups groups of four warps, a group for each 16 rows; they read the same blocks. One
@@ -259,13 +178,14 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
     prefetch_map(&k_map);
     prefetch_map(&v_map);
   }
-  const int64_t total = few_total<kThreads>(a, sh.plan);  // its barriers cover the set-up above
-  const int parts = few_parts(total, gridDim.x);
+  const int64_t total = plan_total<kThreads>(a.batch.sequences, sh.plan, [&](int s) { return few_units(a, s); });  // its barriers cover the set-up above
+  const int parts = plan_parts(total, gridDim.x);
   release_dependents();  // the joining kernel waits for this one's completion by itself
   if (blockIdx.x >= parts) return;
   const int64_t begin = part_begin(total, blockIdx.x, parts);
   const int64_t end = part_begin(total, blockIdx.x + 1, parts);
-  const FewPlace place = few_locate<kThreads>(a, begin, sh.plan);
+  const PlanPlace place =
+      plan_locate<kThreads>(a.batch.sequences, begin, sh.plan, [&](int s) { return few_units(a, s); });
 
   // walk of the part, the same for every role: segments of one (sequence, KV head)
   int s = place.sequence;
@@ -483,7 +403,7 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
     const bool begins = block == 0;
     const bool complete = begins && count == tile.blocks;
     const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (begins ? 1 : 0);
-    const FewPartials<kRows, kDim> partials(a.workspace, gridDim.x);
+    const PartialSums<kRows, kDim> partials(a.workspace, gridDim.x);
     auto joined = [&](int row) {  // (reference, sum) of one of the 16 rows over the warps
       float2 all = make_float2(-INFINITY, 0.0f);
 #pragma unroll
@@ -573,8 +493,9 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
 template <typename T, int kRows, int kDim>
 __global__ void __launch_bounds__(kCombineThreads) paged_attention_few_join_kernel(const PagedAttentionArgs a, int ctas) {
   __shared__ PlanScratch<kCombineThreads> plan;
-  const int64_t total = few_total<kCombineThreads>(a, plan);
-  const int parts = few_parts(total, ctas);
+  const int64_t total =
+      plan_total<kCombineThreads>(a.batch.sequences, plan, [&](int s) { return few_units(a, s); });
+  const int parts = plan_parts(total, ctas);
   const int c = blockIdx.x;  // the boundary between parts c and c + 1
   const int64_t at = part_begin(total, c + 1, max(parts, 1));
   bool cut = c + 1 < parts;
@@ -583,7 +504,8 @@ __global__ void __launch_bounds__(kCombineThreads) paged_attention_few_join_kern
   int kv_head = 0;
   int last = 0;  // part that holds the tile's last unit
   if (cut) {
-    const FewPlace place = few_locate<kCombineThreads>(a, at, plan);
+    const PlanPlace place =
+        plan_locate<kCombineThreads>(a.batch.sequences, at, plan, [&](int s) { return few_units(a, s); });
     seq = paged_sequence(a.batch, place.sequence, nullptr);
     tile = few_tile(seq, a.sliding_window);
     kv_head = static_cast<int>((at - place.before) / tile.blocks);
@@ -596,7 +518,7 @@ __global__ void __launch_bounds__(kCombineThreads) paged_attention_few_join_kern
   if (!cut) return;
   const int group = a.query_heads / a.cache.kv_heads;
   const int rows = seq.q_len * group;
-  const FewPartials<kRows, kDim> partials(a.workspace, ctas);
+  const PartialSums<kRows, kDim> partials(a.workspace, ctas);
   constexpr int kBatch = 8;  // parts whose loads are in flight together
   for (int item = threadIdx.x; item < rows * (kDim / 4); item += kCombineThreads) {
     const int row = item / (kDim / 4);
@@ -647,80 +569,6 @@ __global__ void __launch_bounds__(kCombineThreads) paged_attention_few_join_kern
       a.lse[static_cast<int64_t>(seq.q_begin + token) * a.query_heads + head] =
           sum != 0.0f ? top + log2f(sum) : -INFINITY;
     }
-  }
-}
-
-// ----------------------------------------------------------------------------------- many rows
-constexpr int kRowsThreads = 128;
-
-template <typename T, int kDim>
-__device__ __forceinline__ void load_lane(const T* row, float (&v)[kDim / 32]) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int i = 0; i < kDim / 64; ++i) {
-    const auto pair = reinterpret_cast<const typename Pair<T>::type*>(row)[lane * (kDim / 64) + i];
-    const float2 f = Pair<T>::to_float2(pair);
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
-}
-
-// One warp per row: lane l holds values l * D / 32 .. of q and of the accumulator, a score is a warp
-// sum, and positions the row does not see are never read.
-template <typename T, int kDim>
-__global__ void __launch_bounds__(kRowsThreads) paged_attention_rows_kernel(const PagedAttentionArgs a) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kRowsThreads / 32) + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const int token = static_cast<int>(row / a.query_heads);
-  const int head = static_cast<int>(row - static_cast<int64_t>(token) * a.query_heads);
-  if (token >= a.batch.tokens) return;
-  const int s = paged_sequence_of(a.batch, token);
-  if (s < 0) return;
-  const PagedSequence seq = paged_sequence(a.batch, s, a.status);
-  const int index = token - seq.q_begin;
-  if (index < 0 || index >= seq.q_len) return;
-  const int position = seq.kv_len - seq.q_len + index;
-  const int kv_head = head / (a.query_heads / a.cache.kv_heads);
-  const int first = a.sliding_window > 0 ? max(0, position - a.sliding_window + 1) : 0;
-  constexpr int kValues = kDim / 32;
-  float q[kValues], o[kValues];
-  load_lane<T, kDim>(static_cast<const T*>(a.q) + token * a.q_stride + head * kDim, q);
-#pragma unroll
-  for (int i = 0; i < kValues; ++i) o[i] = 0.0f;
-  float m = -INFINITY, l = 0.0f;
-  const int page_size = 1 << a.cache.page_shift;
-  for (int begin = first; begin <= position;) {
-    const int page = paged_page(a.cache, a.batch, s, begin >> a.cache.page_shift, a.status);
-    const int end = min(position + 1, (begin | (page_size - 1)) + 1);
-    const int64_t base = ((static_cast<int64_t>(page) * a.cache.kv_heads + kv_head) << a.cache.page_shift);
-    for (int j = begin; j < end; ++j) {
-      const int64_t at = (base + (j & (page_size - 1))) * kDim;
-      float k[kValues], v[kValues];
-      load_lane<T, kDim>(static_cast<const T*>(a.cache.k_pages) + at, k);
-      load_lane<T, kDim>(static_cast<const T*>(a.cache.v_pages) + at, v);
-      float dot = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kValues; ++i) dot = fmaf(q[i], k[i], dot);
-      const float x = warp_sum(dot) * a.scale_log2;
-      const float top = fmaxf(m, x);
-      const float keep = exp2f(m - top);  // 0 on the first key
-      const float p = exp2f(x - top);
-      l = l * keep + p;
-#pragma unroll
-      for (int i = 0; i < kValues; ++i) o[i] = o[i] * keep + p * v[i];
-      m = top;
-    }
-    begin = end;
-  }
-  const float inverse = position >= first ? 1.0f / l : 0.0f;
-  T* out = static_cast<T*>(a.out) + token * a.out_stride + head * kDim;
-#pragma unroll
-  for (int i = 0; i < kDim / 64; ++i) {
-    reinterpret_cast<typename Pair<T>::type*>(out)[lane * (kDim / 64) + i] =
-        Pair<T>::from_floats(o[2 * i] * inverse, o[2 * i + 1] * inverse);
-  }
-  if (lane == 0 && a.lse != nullptr) {
-    a.lse[static_cast<int64_t>(token) * a.query_heads + head] = position >= first ? m + log2f(l) : -INFINITY;
   }
 }
 
@@ -789,19 +637,16 @@ cudaError_t launch_dim(const PagedAttentionArgs& a, cudaStream_t stream) {
   const int64_t rows = static_cast<int64_t>(a.batch.max_query) * (a.query_heads / a.cache.kv_heads);
   if (rows <= 16) return launch_few<T, 1, kDim>(a, stream);
   if (rows <= 32) return launch_few<T, 2, kDim>(a, stream);
-  const int64_t all = static_cast<int64_t>(a.batch.tokens) * a.query_heads;
-  paged_attention_rows_kernel<T, kDim>
-      <<<static_cast<unsigned>((all + kRowsThreads / 32 - 1) / (kRowsThreads / 32)), kRowsThreads, 0, stream>>>(a);
-  return cudaGetLastError();
+  return launch_paged_attention_chunk(a, stream);
 }
 
 }  // namespace
 
 int64_t paged_attention_workspace(const PagedCache& cache, const PagedBatch& batch, int query_heads) {
   const int64_t rows = static_cast<int64_t>(batch.max_query) * (query_heads / cache.kv_heads);
-  if (rows <= 16) return few_workspace(16, cache.head_dim, few_ctas<1>());
-  if (rows <= 32) return few_workspace(32, cache.head_dim, few_ctas<2>());
-  return 0;
+  if (rows <= 16) return partial_bytes(16, cache.head_dim, few_ctas<1>());
+  if (rows <= 32) return partial_bytes(32, cache.head_dim, few_ctas<2>());
+  return paged_attention_chunk_workspace(cache.head_dim);
 }
 
 cudaError_t launch_paged_attention(const PagedAttentionArgs& a, cudaStream_t stream) {

@@ -1,0 +1,843 @@
+// Attention of chunks of new tokens over a paged KV cache on tcgen05 / TMEM (contract in
+// include/attnrank_b200.h, formulas in paged_attention.cu).
+//
+// Rows: the query heads of a KV head are stacked, row = token * group + head, so that they share each
+// K and V tile and the causal edge of a tile stays a few tokens wide. A tile is two M = 128 halves of
+// floor(128 / group) tokens each; K and V come in 128-key blocks, one or more pages each, by TMA.
+// One persistent CTA an SM, 384 threads:
+//   warps 0-3, 4-7  softmax of half 0 / 1: thread r owns row r (TMEM lane r) of its half
+//   warp 8          TMA: Q of both halves, K and V blocks into a ring of four stages
+//   warps 9, 10     tcgen05.mma of half 0 / 1 (warp 11 only fills up the warpgroup)
+// TMEM: S0 | S1 | O0 | O1, 128 columns each; P (16-bit) overwrites its S. Per half and block:
+//   S = Q K^T;  softmax warps read S, write P in two halves of 64 keys;  O += P V starts with the first
+//   while the second is being computed;  the next S follows behind it.
+// While one half's products run, the other half's softmax does.
+// Bounds: 4 x 128^3 x 2 FLOP a block and half pair against 2 x 128 x 128 exponentials at 16 a clock and
+// SM: the tensor pipe and the exponentials each take 2048 clocks a block.
+//
+// Work: the (tile, KV head, key block) units form one line that is cut into equal parts, one a CTA
+// (paged_plan.cuh); tiles that a part does not hold whole leave fp32 partial sums, which the joining
+// kernel adds up in order.
+// Masked rows and positions: scores by selection; V values that not every row may see, by clearing the
+// tile's copy (slots past the end, values that are not finite) before the product.
+// Every mbarrier wait is bounded; on expiry the kernel records kStatusWaitTimeout, waits (bounded) for
+// its own MMAs and copies, frees TMEM and returns.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "async_copy.cuh"
+#include "common.cuh"
+#include "layer_kernels.h"
+#include "paged.h"
+#include "paged_plan.cuh"
+#include "tensor_core.cuh"
+
+namespace arb {
+namespace {
+
+using namespace async;
+using namespace tc;
+
+constexpr int kRows = 128;                          // rows of a half tile
+constexpr int kThreads = 384;
+// setmaxnreg shares of the 384 x 168 registers of the launch: 256 x 208 + 128 x 80 = 63488 <= 64512
+constexpr int kSoftmaxRegisters = 208;
+constexpr int kIssueRegisters = 80;
+constexpr int kStages = 4;
+constexpr uint32_t kHalfBytes = 128 * 128;          // 128 rows of 64 16-bit values
+constexpr uint32_t kTmemColumns = 512;
+constexpr uint32_t kTmemO = 256;
+constexpr int kJoinThreads = 256;
+constexpr int kJoinRows = 32;                       // rows of a tile that one joining CTA takes
+constexpr float kRescaleThreshold = 8.0f;           // log2 units
+constexpr int kChains = 4;                          // independent accumulators per row reduction
+
+struct __align__(16) Control {
+  uint64_t q_full;
+  uint64_t q_empty;
+  uint64_t full[kStages];
+  uint64_t empty[kStages];
+  uint64_t s_full[2];
+  uint64_t p_full[2][2];
+  uint64_t o_full[2];
+  uint64_t o_free[2];
+  uint64_t clean[2];
+  uint64_t done[2];
+  uint32_t tmem_base;
+  volatile int abort;
+  unsigned poison;  // bit segment % 32: V held a value that is not finite where some row may not look
+  PlanScratch<kThreads> plan;
+};
+
+template <int kDim>
+struct Layout {
+  static constexpr uint32_t kOperand = kHalfBytes * (kDim / 64);  // 128 rows of K, V, or half a tile's Q
+  static constexpr uint32_t kRing = 2 * kOperand;
+  static constexpr uint32_t kControl = kRing + kStages * kOperand;
+  static constexpr size_t bytes() { return kControl + sizeof(Control) + 1024; }
+};
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+struct ChunkArgs {
+  PagedAttentionArgs a;
+  int half_tokens;  // tokens of half a tile
+  uint32_t idesc_s;
+  uint32_t idesc_o;
+};
+
+__device__ __forceinline__ int64_t chunk_units(const ChunkArgs& c, int s) {
+  const PagedSequence seq = paged_sequence(c.a.batch, s, c.a.status);
+  return chunk_blocks(seq.q_len, seq.kv_len, 2 * c.half_tokens, c.a.sliding_window) * c.a.cache.kv_heads;
+}
+
+// A place in the line: block `block` of tile `t`, KV head `kv_head`, sequence `s`.
+struct ChunkPlace {
+  int s, t, kv_head, block;
+  int64_t tile_begin;  // the line's unit at which (sequence, tile, KV head) begins
+};
+
+template <int kCount>
+__device__ __forceinline__ ChunkPlace chunk_locate(const ChunkArgs& c, int64_t unit, PlanScratch<kCount>& scratch) {
+  const PlanPlace place = plan_locate<kCount>(c.a.batch.sequences, unit, scratch, [&](int s) { return chunk_units(c, s); });
+  const PagedSequence seq = paged_sequence(c.a.batch, place.sequence, nullptr);
+  const int step = 2 * c.half_tokens;
+  const int tiles = (seq.q_len + step - 1) / step;
+  __syncthreads();  // `place` has been read by everyone
+  const PlanPlace in = plan_locate<kCount>(tiles, unit - place.before, scratch, [&](int t) {
+    return static_cast<int64_t>(chunk_tile(seq.q_len, seq.kv_len, step, c.a.sliding_window, t).blocks) * c.a.cache.kv_heads;
+  });
+  const int blocks = chunk_tile(seq.q_len, seq.kv_len, step, c.a.sliding_window, in.sequence).blocks;
+  const int64_t rest = unit - place.before - in.before;
+  ChunkPlace out;
+  out.s = place.sequence;
+  out.t = in.sequence;
+  out.kv_head = static_cast<int>(rest / blocks);
+  out.block = static_cast<int>(rest - static_cast<int64_t>(out.kv_head) * blocks);
+  out.tile_begin = unit - out.block;
+  return out;
+}
+
+// One segment: the part of a (tile, KV head) that one CTA does.
+struct Walk {
+  PagedSequence seq;
+  ChunkTile tile;
+  int s, t, kv_head;
+  int block;     // first block of the segment, relative to the tile's
+  int count;     // its blocks
+  int64_t left;  // units of the part from this segment on
+  // blocks of the segment [begin, end) that any row of a half sees, relative to the tile's
+  __device__ __forceinline__ void half_range(int half, int half_tokens, int window, int& begin, int& end) const {
+    const int first = tile.first_position + half * half_tokens;
+    const int last = min(first + half_tokens - 1, tile.last_position);
+    begin = end = block;
+    if (first > tile.last_position || last < 0) return;
+    const int first_key = window > 0 && first >= window ? first - window + 1 : 0;
+    begin = max(block, first_key / kChunkBlock - tile.block_begin);
+    end = max(begin, min(block + count, last / kChunkBlock + 1 - tile.block_begin));
+  }
+  // does every row of the tile see every key of block b?
+  __device__ __forceinline__ bool whole(int b, int window) const {
+    const int key = (tile.block_begin + b) * kChunkBlock;
+    return key + kChunkBlock - 1 <= tile.first_position && (window == 0 || key > tile.last_position - window);
+  }
+};
+
+__device__ __forceinline__ void walk_tile(Walk& w, const ChunkArgs& c) {
+  w.tile = chunk_tile(w.seq.q_len, w.seq.kv_len, 2 * c.half_tokens, c.a.sliding_window, w.t);
+  w.count = static_cast<int>(min(w.left, static_cast<int64_t>(w.tile.blocks - w.block)));
+}
+__device__ __forceinline__ bool walk_next(Walk& w, const ChunkArgs& c) {
+  w.left -= w.count;
+  if (w.left <= 0) return false;
+  w.block = 0;
+  if (++w.kv_head == c.a.cache.kv_heads) {
+    w.kv_head = 0;
+    if (++w.t * 2 * c.half_tokens >= w.seq.q_len) {
+      w.t = 0;
+      do {  // units remain, so a sequence with new tokens follows
+        w.seq = paged_sequence(c.a.batch, ++w.s, nullptr);
+      } while (w.seq.q_len == 0 && w.s + 1 < c.a.batch.sequences);
+    }
+  }
+  walk_tile(w, c);
+  return true;
+}
+
+template <typename T>
+__device__ __forceinline__ bool nonfinite_half(uint32_t bits) {
+  constexpr uint32_t kExponent = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
+  return (bits & kExponent) == kExponent;
+}
+
+// Sum of the values of column `column` that are not finite, over the keys [first, last] of sequence s.
+template <typename T, int kDim>
+__device__ __noinline__ float nonfinite_sum(const PagedAttentionArgs& a, int s, int kv_head, int first, int last,
+                                            int column) {
+  float sum = 0.0f;
+  for (int key = first; key <= last; ++key) {
+    const int page = paged_page(a.cache, a.batch, s, key >> a.cache.page_shift, a.status);
+    const int64_t row = ((static_cast<int64_t>(page) * a.cache.kv_heads + kv_head) << a.cache.page_shift) +
+                        (key & ((1 << a.cache.page_shift) - 1));
+    const float v = static_cast<float>(static_cast<const T*>(a.cache.v_pages)[row * kDim + column]);
+    if (!isfinite(v)) sum += v;
+  }
+  return sum;
+}
+
+template <typename T, int kDim>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                                 const __grid_constant__ CUtensorMap v_map, const ChunkArgs c) {
+  constexpr uint32_t kOperand = Layout<kDim>::kOperand;
+  constexpr int kHalves = kDim / 64;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Control& ctl = *reinterpret_cast<Control*>(smem + Layout<kDim>::kControl);
+  const uint32_t q_smem = smem_u32(smem);
+  const uint32_t ring = q_smem + Layout<kDim>::kRing;
+  const PagedAttentionArgs& a = c.a;
+  const int tid = threadIdx.x;
+  const int warp = tid >> 5;
+  const int lane = tid & 31;
+  const int window = a.sliding_window;
+
+  if (tid == 0) {
+    mbar_init(smem_u32(&ctl.q_full), 1);
+    mbar_init(smem_u32(&ctl.q_empty), 2);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(smem_u32(&ctl.full[i]), 1);
+      mbar_init(smem_u32(&ctl.empty[i]), 2);
+    }
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(smem_u32(&ctl.s_full[h]), 1);
+      mbar_init(smem_u32(&ctl.p_full[h][0]), kRows);
+      mbar_init(smem_u32(&ctl.p_full[h][1]), kRows);
+      mbar_init(smem_u32(&ctl.o_full[h]), 1);
+      mbar_init(smem_u32(&ctl.o_free[h]), kRows);
+      mbar_init(smem_u32(&ctl.clean[h]), 2 * kRows);
+      mbar_init(smem_u32(&ctl.done[h]), 1);
+    }
+    ctl.abort = 0;
+    ctl.poison = 0;
+    mbar_init_fence();
+    prefetch_map(&q_map);
+    prefetch_map(&k_map);
+    prefetch_map(&v_map);
+  }
+  // the part of this CTA (the barriers inside also cover the set-up above)
+  const int64_t total =
+      plan_total<kThreads>(a.batch.sequences, ctl.plan, [&](int s) { return chunk_units(c, s); });
+  const int parts = plan_parts(total, gridDim.x);
+  release_dependents();  // the joining kernel waits for this one's completion by itself
+  if (blockIdx.x >= parts) return;
+  const int64_t begin = part_begin(total, blockIdx.x, parts);
+  Walk w;
+  {
+    const ChunkPlace place = chunk_locate<kThreads>(c, begin, ctl.plan);
+    w.s = place.s;
+    w.t = place.t;
+    w.kv_head = place.kv_head;
+    w.block = place.block;
+    w.left = part_begin(total, blockIdx.x + 1, parts) - begin;
+    w.seq = paged_sequence(a.batch, w.s, nullptr);
+    walk_tile(w, c);
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_base)),
+                 "r"(kTmemColumns));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = ctl.tmem_base;
+  const int group = a.query_heads / a.cache.kv_heads;
+  const int half_tokens = c.half_tokens;
+  // Ring item 2n is K of the part's n-th block, item 2n + 1 its V: stage item % 4, phase item / 4.
+  auto stage_of = [](uint32_t item) { return item % kStages; };
+  auto phase_of = [](uint32_t item) { return (item / kStages) & 1; };
+  bool ok = true;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegisters));
+  if (warp == 8) {
+    // ------------------------------------------------------------------------------------- TMA
+    const int page_rows = min(1 << a.cache.page_shift, kChunkBlock);
+    const int boxes = kChunkBlock / page_rows * kHalves;
+    const int my_page = lane / kHalves;  // the lane's box: page and 64-wide half
+    const int my_half = lane - my_page * kHalves;
+    uint32_t item = 0;
+    uint32_t segment = 0;
+    do {
+      if (segment > 0 && !mbar_wait(smem_u32(&ctl.q_empty), (segment - 1) & 1, &ctl.abort)) {
+        ok = false;
+        break;
+      }
+      const int first_token = w.t * 2 * half_tokens;
+      const int q_halves = first_token + half_tokens < w.seq.q_len ? 2 : 1;
+      const uint32_t q_bar = smem_u32(&ctl.q_full);
+      if (lane == 0) mbar_expect_tx(q_bar, q_halves * kHalves * half_tokens * group * 128);
+      __syncwarp();
+      if (lane < q_halves * kHalves) {
+        const int half = lane / kHalves;
+        const int column = lane - half * kHalves;
+        tma_load_3d(q_smem + half * kOperand + column * kHalfBytes, &q_map, column * 64, w.kv_head * group,
+                    w.seq.q_begin + first_token + half * half_tokens, q_bar);
+      }
+      ++segment;
+      const int key_end = w.tile.last_position + 1;
+      auto page_at = [&](int b) {  // the lane's page of block b, -1 when no row needs it
+        const int key = (w.tile.block_begin + b) * kChunkBlock + my_page * page_rows;
+        if (lane >= boxes || key >= key_end || key + page_rows <= w.tile.first_key) return -1;
+        return paged_page(a.cache, a.batch, w.s, key >> a.cache.page_shift, a.status);
+      };
+      int page = page_at(w.block);
+      for (int i = 0; i < w.count; ++i) {
+        const int following = i + 1 < w.count ? page_at(w.block + i + 1) : -1;  // hides behind the waits
+        const uint32_t loads = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        const int key = (w.tile.block_begin + w.block + i) * kChunkBlock + my_page * page_rows;
+        const int row = ((page * a.cache.kv_heads + w.kv_head) << a.cache.page_shift) +
+                        (key & ((1 << a.cache.page_shift) - 1));
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv, ++item) {
+          const uint32_t stage = stage_of(item);
+          if (item >= kStages && !mbar_wait(smem_u32(&ctl.empty[stage]), phase_of(item) ^ 1, &ctl.abort)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = smem_u32(&ctl.full[stage]);
+          if (lane == 0) mbar_expect_tx(bar, loads * page_rows * 128);
+          __syncwarp();
+          if (page >= 0) {
+            tma_load_2d(ring + stage * kOperand + my_half * kHalfBytes + my_page * page_rows * 128,
+                        kv == 0 ? &k_map : &v_map, my_half * 64, row, bar);
+          }
+        }
+        if (!ok) break;
+        page = following;
+      }
+    } while (ok && walk_next(w, c));
+    if (!ok) {
+      if (lane == 0) {
+        report_status(a.status, kStatusWaitTimeout);
+        ctl.abort = 1;
+      }
+      // the loads in flight land before the shared memory is released
+      if (segment > 0) mbar_wait(smem_u32(&ctl.q_full), (segment - 1) & 1, nullptr);
+      for (uint32_t i = item > kStages ? item - kStages : 0; i < item; ++i) {
+        mbar_wait(smem_u32(&ctl.full[stage_of(i)]), phase_of(i), nullptr);
+      }
+    }
+  } else if (warp > 8) {
+    // ------------------------------------------------------------------------------------- MMA
+    const int half = warp - 9;
+    if (lane == 0 && half < 2) {
+      const uint32_t s_tmem = tmem + half * 128;
+      const uint32_t o_tmem = tmem + kTmemO + half * 128;
+      const uint32_t q_at = q_smem + half * kOperand;
+      uint32_t turn = 0;  // blocks so far
+      uint32_t segment = 0;
+      uint32_t cleaned[2] = {0, 0};
+      do {
+        int h_begin, h_end;
+        w.half_range(half, half_tokens, window, h_begin, h_end);
+        const int end = w.block + w.count;
+        ok = mbar_wait(smem_u32(&ctl.q_full), segment & 1, &ctl.abort);
+        if (!ok) break;
+        // K of block b: S = Q K^T when the half needs it; the stage is released either way
+        auto do_scores = [&](int b, uint32_t n) {
+          const uint32_t stage = stage_of(2 * n);
+          const bool needed = b >= h_begin && b < h_end;
+          // also without need: a release before the fill would count for the stage's use before
+          if (!mbar_wait(smem_u32(&ctl.full[stage]), phase_of(2 * n), &ctl.abort)) return false;
+          if (needed) {
+            fence_after();
+            const uint32_t k_at = ring + stage * kOperand;
+#pragma unroll
+            for (int k = 0; k < kDim / 16; ++k) {
+              const uint32_t offset = (k >> 2) * kHalfBytes + (k & 3) * 32;
+              mma_ss(s_tmem, desc_k_major(q_at + offset), desc_k_major(k_at + offset), c.idesc_s, k > 0 ? 1u : 0u);
+            }
+            mma_commit(smem_u32(&ctl.s_full[half]));
+            mma_commit(smem_u32(&ctl.empty[stage]));
+          } else {
+            mbar_arrive(smem_u32(&ctl.s_full[half]));
+            mbar_arrive(smem_u32(&ctl.empty[stage]));
+          }
+          // Q has been read for the last time by this half
+          if (needed ? b == h_end - 1 : (h_begin == h_end && b == end - 1)) mma_commit(smem_u32(&ctl.q_empty));
+          return true;
+        };
+        ok = do_scores(w.block, turn);
+        if (!ok) break;
+        bool waited_o = segment == 0;
+        for (int b = w.block; b < end; ++b, ++turn) {
+          const uint32_t v_item = 2 * turn + 1;
+          const uint32_t stage = stage_of(v_item);
+          const bool needed = b >= h_begin && b < h_end;
+          const bool whole = w.whole(b, window);
+          if (needed && !waited_o) {  // the last segment's O has been read
+            ok = mbar_wait(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
+            waited_o = true;
+          }
+          ok = ok && mbar_wait(smem_u32(&ctl.full[stage]), phase_of(v_item), &ctl.abort);
+          if (ok && !whole) {  // V of this block is cleared by the softmax warps first
+            ok = mbar_wait(smem_u32(&ctl.clean[turn & 1]), cleaned[turn & 1] & 1, &ctl.abort);
+            ++cleaned[turn & 1];
+          }
+          if (!ok) break;
+          const uint32_t v_at = ring + stage * kOperand;
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            ok = ok && mbar_wait(smem_u32(&ctl.p_full[half][part]), turn & 1, &ctl.abort);
+            if (ok && needed) {
+              fence_after();
+#pragma unroll
+              for (int k = part * 4; k < part * 4 + 4; ++k) {
+                mma_ts(o_tmem, s_tmem + k * 8, desc_mn_major(v_at + k * 16 * 128, kHalfBytes), c.idesc_o,
+                       (b > h_begin || k > 0) ? 1u : 0u);
+              }
+            }
+          }
+          if (!ok) break;
+          if (needed) {
+            mma_commit(smem_u32(&ctl.empty[stage]));
+            mma_commit(smem_u32(&ctl.o_full[half]));
+          } else {
+            mbar_arrive(smem_u32(&ctl.empty[stage]));
+          }
+          if (b + 1 < end) ok = do_scores(b + 1, turn + 1);
+          if (!ok) break;
+        }
+        if (!ok) break;
+        if (!waited_o) {
+          ok = mbar_wait(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
+          if (!ok) break;
+        }
+        // a half without blocks takes part too, so that its softmax warps stay within a segment of it
+        if (h_begin == h_end) mbar_arrive(smem_u32(&ctl.o_full[half]));
+        ++segment;
+      } while (walk_next(w, c));
+      if (!ok) {
+        report_status(a.status, kStatusWaitTimeout);
+        ctl.abort = 1;
+      }
+      // every MMA of this thread has completed before TMEM and shared memory are released
+      mma_commit(smem_u32(&ctl.done[half]));
+      mbar_wait(smem_u32(&ctl.done[half]), 0, nullptr);
+    }
+    __syncwarp();
+  }
+  } else {
+    // --------------------------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
+    const int half = warp >> 2;
+    const int row = tid & (kRows - 1);
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_tmem = tmem + half * 128 + lane_base;
+    const uint32_t o_tmem = tmem + kTmemO + half * 128 + lane_base;
+    const int row_token = row / group;
+    const int row_head = row - row_token * group;
+    const PartialSums<2 * kRows, kDim> partials(a.workspace, gridDim.x);
+    uint32_t turn = 0;
+    uint32_t outputs = 0;  // phases of o_full so far: one a block, one a segment without any
+    uint32_t segment = 0;
+    uint32_t cleaned[2] = {0, 0};
+    do {
+      int h_begin, h_end;
+      w.half_range(half, half_tokens, window, h_begin, h_end);
+      const int end = w.block + w.count;
+      const int token = w.t * 2 * half_tokens + half * half_tokens + row_token;
+      const bool row_in = row_token < half_tokens && token < w.seq.q_len;
+      const int position = w.seq.kv_len - w.seq.q_len + token;
+      const int row_first = window > 0 && position >= window ? position - window + 1 : 0;
+      const int row_last = row_in ? position : -1;
+      if (tid == 0) atomicAnd(&ctl.poison, ~(1u << ((segment + 16) & 31)));  // the halves are never 16 segments apart
+      float reference = -INFINITY;
+      float l = 0.0f;
+      // tcgen05.ld / tcgen05.st are warp-collective: every branch around them is uniform per warp
+      for (int b = w.block; b < end; ++b, ++turn) {
+        const bool needed = b >= h_begin && b < h_end;
+        const bool whole = w.whole(b, window);
+        const int key0 = (w.tile.block_begin + b) * kChunkBlock;
+        // every block passes through s_full and p_full, needed by the half or not, so that neither side
+        // is ever more than one phase ahead of a barrier that it waits on
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl.s_full[half]), turn & 1, &ctl.abort));
+        if (!ok) break;
+        if (!whole) {
+          // Clear what no row of the tile sees, and values that are not finite (a probability of zero
+          // times one would be NaN); the rows that see those get them added at the end.
+          const uint32_t v_item = 2 * turn + 1;
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait(smem_u32(&ctl.full[stage_of(v_item)]), phase_of(v_item), &ctl.abort));
+          if (!ok) break;
+          uint4* v = reinterpret_cast<uint4*>(smem + Layout<kDim>::kRing + stage_of(v_item) * kOperand);
+          bool bad = false;
+#pragma unroll 4
+          for (int i = tid; i < static_cast<int>(kOperand / 16); i += 2 * kRows) {
+            const int key = key0 + ((i >> 3) & (kChunkBlock - 1));  // eight chunks of 16 bytes a row
+            const bool in = key >= w.tile.first_key && key <= w.tile.last_position;
+            uint4 value = v[i];
+            uint32_t* words = reinterpret_cast<uint32_t*>(&value);
+            bool change = !in;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const bool low = nonfinite_half<T>(words[j]);
+              const bool high = nonfinite_half<T>(words[j] >> 16);
+              bad |= in && (low || high);
+              change |= low || high;
+              words[j] = in ? (low ? 0u : words[j] & 0xffffu) | (high ? 0u : words[j] & 0xffff0000u) : 0u;
+            }
+            if (change) v[i] = value;
+          }
+          if (bad) atomicOr(&ctl.poison, 1u << (segment & 31));
+          fence_async_shared();
+          mbar_arrive(smem_u32(&ctl.clean[turn & 1]));
+          ++cleaned[turn & 1];
+          __syncwarp();
+        }
+        if (!needed) {
+          mbar_arrive(smem_u32(&ctl.p_full[half][0]));
+          mbar_arrive(smem_u32(&ctl.p_full[half][1]));
+          continue;
+        }
+        fence_after();
+        float x[kChunkBlock];
+        {
+          uint32_t raw[4][32];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tmem_ld32(s_tmem + i * 32, raw[i]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < kChunkBlock; ++i) x[i] = __uint_as_float(raw[i >> 5][i & 31]);
+        }
+        if (!whole) {
+          const int low = row_first - key0;
+          const int high = row_last - key0;
+#pragma unroll
+          for (int i = 0; i < kChunkBlock; ++i) {
+            if (i < low || i > high) x[i] = -INFINITY;
+          }
+        }
+        float top[kChains];
+#pragma unroll
+        for (int i = 0; i < kChains; ++i) top[i] = x[i];
+#pragma unroll
+        for (int i = kChains; i < kChunkBlock; i += 2) {
+          top[(i / 2) % kChains] = max3(top[(i / 2) % kChains], x[i], x[i + 1]);
+        }
+        const float block_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+        // the row's reference moves only when the block's maximum exceeds it by more than the threshold,
+        // so probabilities stay below 2^8 and O is rarely rescaled
+        const bool move = block_top > reference + kRescaleThreshold || (reference == -INFINITY && block_top != -INFINITY);
+        const bool rescale = move && reference != -INFINITY;
+        if (__any_sync(0xffffffffu, rescale)) {
+          // O holds the segment's blocks before this one
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl.o_full[half]), (outputs - 1) & 1, &ctl.abort));
+          if (!ok) break;
+          fence_after();
+          const float factor = rescale ? ex2_ftz(reference - block_top) : 1.0f;
+#pragma unroll 1
+          for (int i = 0; i < kDim / 32; ++i) {
+            uint32_t raw[32];
+            tmem_ld32(o_tmem + i * 32, raw);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) raw[j] = __float_as_uint(__uint_as_float(raw[j]) * factor);
+            tmem_st32(o_tmem + i * 32, raw);
+          }
+          l *= factor;
+        }
+        if (move) reference = block_top;
+        const float base = reference == -INFINITY ? 0.0f : -reference;
+        const unsigned long long scale2 = pack_f32x2(a.scale_log2, a.scale_log2);
+        const unsigned long long base2 = pack_f32x2(base, base);
+        unsigned long long sums[kChains / 2];
+#pragma unroll
+        for (int i = 0; i < kChains / 2; ++i) sums[i] = 0ull;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          uint32_t packed[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int at = part * 64 + 2 * i;
+            float t0, t1;
+            unpack_f32x2(fma_f32x2(pack_f32x2(x[at], x[at + 1]), scale2, base2), t0, t1);
+            const float p0 = ex2_ftz(t0);
+            const float p1 = ex2_ftz(t1);
+            sums[i % (kChains / 2)] = add_f32x2(sums[i % (kChains / 2)], pack_f32x2(p0, p1));
+            packed[i] = pack2<T>(p0, p1);
+          }
+          tmem_st32(s_tmem + part * 32, packed);
+          tmem_wait_st();
+          fence_before();
+          mbar_arrive(smem_u32(&ctl.p_full[half][part]));
+        }
+#pragma unroll
+        for (int i = 0; i < kChains / 2; ++i) {
+          float s0, s1;
+          unpack_f32x2(sums[i], s0, s1);
+          l += s0 + s1;
+        }
+        ++outputs;
+      }
+      if (!ok) break;
+      // ---- the segment's rows: O / l, or the partial sums
+      const bool any = h_end > h_begin;
+      if (!any) ++outputs;
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl.o_full[half]), (outputs - 1) & 1, &ctl.abort));
+      if (!ok) break;
+      fence_after();
+      // every thread's share of the cleared blocks is done when their barriers' last phases are
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (cleaned[i] > 0 && ok) {
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl.clean[i]), (cleaned[i] - 1) & 1, &ctl.abort));
+        }
+      }
+      if (!ok) break;
+      const bool poisoned = (*reinterpret_cast<volatile unsigned*>(&ctl.poison) >> (segment & 31)) & 1;
+      const bool begins = w.block == 0;
+      const bool complete = begins && w.count == w.tile.blocks;
+      const float factor = complete ? (l != 0.0f ? 1.0f / l : 0.0f) : 1.0f;
+      const int head = w.kv_head * group + row_head;
+      const int64_t slot_row = (static_cast<int64_t>(blockIdx.x) * 2 + (begins ? 1 : 0)) * (2 * kRows) + half * kRows + row;
+      const int64_t out_token = w.seq.q_begin + token;
+#pragma unroll 1
+      for (int i = 0; i < kDim / 32; ++i) {
+        uint32_t raw[32];
+        __syncwarp();  // rows of a warp part below
+        if (any) {
+          tmem_ld32(o_tmem + i * 32, raw);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) raw[j] = 0u;
+        }
+        if (row_in && poisoned) {
+          const int low = max(row_first, (w.tile.block_begin + w.block) * kChunkBlock);
+          const int high = min(row_last, (w.tile.block_begin + end) * kChunkBlock - 1);
+          for (int j = 0; j < 32; ++j) {
+            const float more = nonfinite_sum<T, kDim>(a, w.s, w.kv_head, low, high, i * 32 + j);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              if (k == j) raw[k] = __float_as_uint(__uint_as_float(raw[k]) + more);
+            }
+          }
+        }
+        if (row_in && complete) {
+          T* to = static_cast<T*>(a.out) + out_token * a.out_stride + head * kDim + i * 32;
+          uint32_t packed[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            packed[j] = pack2<T>(__uint_as_float(raw[2 * j]) * factor, __uint_as_float(raw[2 * j + 1]) * factor);
+          }
+          uint4* to16 = reinterpret_cast<uint4*>(to);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            to16[j] = make_uint4(packed[4 * j], packed[4 * j + 1], packed[4 * j + 2], packed[4 * j + 3]);
+          }
+        } else if (row_in) {
+          float4* to = reinterpret_cast<float4*>(partials.sums + slot_row * kDim + i * 32);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            to[j] = make_float4(__uint_as_float(raw[4 * j]), __uint_as_float(raw[4 * j + 1]),
+                                __uint_as_float(raw[4 * j + 2]), __uint_as_float(raw[4 * j + 3]));
+          }
+        }
+      }
+      __syncwarp();
+      fence_before();
+      mbar_arrive(smem_u32(&ctl.o_free[half]));
+      if (row_in) {
+        if (!complete) {
+          partials.stats[slot_row] = make_float2(reference, l);
+        } else if (a.lse != nullptr) {
+          a.lse[out_token * a.query_heads + head] = l != 0.0f ? reference + log2f(l) : -INFINITY;
+        }
+      }
+      __syncwarp();
+      ++segment;
+    } while (walk_next(w, c));
+    if (!ok && lane == 0) {
+      report_status(a.status, kStatusWaitTimeout);
+      ctl.abort = 1;
+    }
+  }
+
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns));
+  }
+}
+
+// Joins the parts of the tile that the boundary between CTAs c and c + 1 cuts, for the first such
+// boundary of each tile, in the order of the CTAs; blockIdx.y: kJoinRows of the tile's rows.
+template <typename T, int kDim>
+__global__ void __launch_bounds__(kJoinThreads) paged_attention_chunk_join_kernel(const ChunkArgs c, int ctas) {
+  __shared__ PlanScratch<kJoinThreads> plan;
+  const PagedAttentionArgs& a = c.a;
+  const int64_t total = plan_total<kJoinThreads>(a.batch.sequences, plan, [&](int s) { return chunk_units(c, s); });
+  const int parts = plan_parts(total, ctas);
+  const int boundary = blockIdx.x;
+  bool cut = boundary + 1 < parts;
+  ChunkPlace place{};
+  PagedSequence seq{};
+  int last = 0;  // part that holds the tile's last unit
+  if (cut) {
+    const int64_t at = part_begin(total, boundary + 1, parts);
+    place = chunk_locate<kJoinThreads>(c, at, plan);
+    seq = paged_sequence(a.batch, place.s, nullptr);
+    const int blocks = chunk_tile(seq.q_len, seq.kv_len, 2 * c.half_tokens, a.sliding_window, place.t).blocks;
+    cut = place.block > 0 && part_begin(total, boundary, parts) <= place.tile_begin;
+    last = part_of(total, place.tile_begin + blocks - 1, parts);
+  }
+  // every CTA waits, so that this grid does not complete before the one whose sums it reads
+  wait_for_producer();
+  if (!cut) return;
+  const int group = a.query_heads / a.cache.kv_heads;
+  const PartialSums<2 * kRows, kDim> partials(a.workspace, ctas);
+  constexpr int kBatch = 4;  // parts whose loads are in flight together
+  for (int item = threadIdx.x; item < kJoinRows * (kDim / 4); item += kJoinThreads) {
+    const int tile_row = blockIdx.y * kJoinRows + item / (kDim / 4);
+    const int column = item % (kDim / 4) * 4;
+    const int half = tile_row / kRows;
+    const int row = tile_row - half * kRows;
+    const int row_token = row / group;
+    const int token = (place.t * 2 + half) * c.half_tokens + row_token;
+    if (row_token >= c.half_tokens || token >= seq.q_len) continue;
+    float top = -INFINITY;
+    float sum = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int first = boundary; first <= last; first += kBatch) {
+      float2 stats[kBatch];
+      float4 piece[kBatch];
+      float high = top;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int part = first + i;
+        stats[i] = make_float2(-INFINITY, 0.0f);
+        piece[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (part <= last) {
+          const int64_t at_row = (static_cast<int64_t>(part) * 2 + (part == boundary ? 1 : 0)) * (2 * kRows) + tile_row;
+          stats[i] = partials.stats[at_row];
+          piece[i] = *reinterpret_cast<const float4*>(partials.sums + at_row * kDim + column);
+        }
+        high = fmaxf(high, stats[i].x);
+      }
+      const float keep = top == -INFINITY ? 0.0f : ex2_ftz(top - high);
+      sum *= keep;
+      o.x *= keep;
+      o.y *= keep;
+      o.z *= keep;
+      o.w *= keep;
+      top = high;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const float factor = stats[i].x == -INFINITY ? 0.0f : ex2_ftz(stats[i].x - top);
+        sum += factor * stats[i].y;
+        o.x += factor * piece[i].x;
+        o.y += factor * piece[i].y;
+        o.z += factor * piece[i].z;
+        o.w += factor * piece[i].w;
+      }
+    }
+    const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
+    const int head = place.kv_head * group + row - row_token * group;
+    T* to = static_cast<T*>(a.out) + (seq.q_begin + token) * a.out_stride + head * kDim + column;
+    *reinterpret_cast<uint2*>(to) =
+        make_uint2(pack2<T>(o.x * inverse, o.y * inverse), pack2<T>(o.z * inverse, o.w * inverse));
+    if (column == 0 && a.lse != nullptr) {
+      a.lse[static_cast<int64_t>(seq.q_begin + token) * a.query_heads + head] =
+          sum != 0.0f ? top + log2f(sum) : -INFINITY;
+    }
+  }
+}
+
+template <typename T>
+bool encode_map(CUtensorMap* map, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+                const cuuint32_t* box) {
+  PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
+  if (encode == nullptr) return false;
+  const cuuint32_t element_strides[3] = {1, 1, 1};
+  const CUtensorMapDataType type =
+      std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return encode(map, type, rank, const_cast<void*>(base), dims, strides, box, element_strides,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int kDim>
+cudaError_t launch_chunk(const PagedAttentionArgs& a, cudaStream_t stream) {
+  static_assert(Layout<kDim>::bytes() <= 227 * 1024, "one CTA's shared memory");
+  int device = 0;
+  cudaGetDevice(&device);
+  static uint64_t configured = 0;  // the shared-memory opt-in is a per-device attribute
+  if (device >= 64 || !(configured & (1ull << device))) {
+    const cudaError_t status =
+        cudaFuncSetAttribute(paged_attention_chunk_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(Layout<kDim>::bytes()));
+    if (status != cudaSuccess) return status;
+    if (device < 64) configured |= 1ull << device;
+  }
+  const int group = a.query_heads / a.cache.kv_heads;
+  ChunkArgs c;
+  c.a = a;
+  c.half_tokens = kRows / group;
+  const uint32_t format = std::is_same_v<T, __half> ? 0u : 1u;
+  c.idesc_s = idesc(format, false, kChunkBlock);
+  c.idesc_o = idesc(format, true, kDim);
+  CUtensorMap q_map, k_map, v_map;
+  // Q: (64 values, the group's heads, half a tile's tokens); rows past the call's are zeros
+  const cuuint64_t q_dims[3] = {kDim, static_cast<cuuint64_t>(a.query_heads), static_cast<cuuint64_t>(a.batch.tokens)};
+  const cuuint64_t q_strides[2] = {kDim * 2, static_cast<cuuint64_t>(a.q_stride) * 2};
+  const cuuint32_t q_box[3] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(c.half_tokens)};
+  const cuuint64_t pool_rows = (static_cast<cuuint64_t>(a.cache.page_count) * a.cache.kv_heads) << a.cache.page_shift;
+  const cuuint64_t dims[2] = {kDim, pool_rows};
+  const cuuint64_t strides[1] = {kDim * 2};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(std::min(1 << a.cache.page_shift, kChunkBlock))};
+  if (!encode_map<T>(&q_map, 3, a.q, q_dims, q_strides, q_box) ||
+      !encode_map<T>(&k_map, 2, a.cache.k_pages, dims, strides, box) ||
+      !encode_map<T>(&v_map, 2, a.cache.v_pages, dims, strides, box)) {
+    return cudaErrorInvalidValue;
+  }
+  const int ctas = sm_count();
+  paged_attention_chunk_kernel<T, kDim><<<ctas, kThreads, Layout<kDim>::bytes(), stream>>>(q_map, k_map, v_map, c);
+  cudaError_t status = cudaGetLastError();
+  if (status != cudaSuccess || ctas < 2) return status;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(ctas - 1, 2 * kRows / kJoinRows);
+  config.blockDim = dim3(kJoinThreads);
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  status = cudaLaunchKernelEx(&config, paged_attention_chunk_join_kernel<T, kDim>, c, ctas);
+  return status != cudaSuccess ? status : cudaGetLastError();
+}
+
+}  // namespace
+
+int64_t paged_attention_chunk_workspace(int head_dim) { return partial_bytes(2 * kRows, head_dim, sm_count()); }
+
+cudaError_t launch_paged_attention_chunk(const PagedAttentionArgs& a, cudaStream_t stream) {
+  if (a.cache.dtype == kActFp16) {
+    return a.cache.head_dim == 128 ? launch_chunk<__half, 128>(a, stream) : launch_chunk<__half, 64>(a, stream);
+  }
+  return a.cache.head_dim == 128 ? launch_chunk<__nv_bfloat16, 128>(a, stream)
+                                 : launch_chunk<__nv_bfloat16, 64>(a, stream);
+}
+
+}  // namespace arb
