@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t ring = q_smem + Layout<kDim>::kRing;
   const PagedAttentionArgs& a = c.a;
   const int tid = threadIdx.x;
-  const int warp = tid >> 5;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be the same in the whole warp
   const int lane = tid & 31;
   const int window = a.sliding_window;
 
@@ -217,11 +217,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int h = 0; h < 2; ++h) {
       mbar_init(smem_u32(&ctl.s_full[h]), 1);
-      mbar_init(smem_u32(&ctl.p_full[h][0]), kRows);
-      mbar_init(smem_u32(&ctl.p_full[h][1]), kRows);
+      mbar_init(smem_u32(&ctl.p_full[h][0]), 4);  // one arrival a softmax warp
+      mbar_init(smem_u32(&ctl.p_full[h][1]), 4);
       mbar_init(smem_u32(&ctl.o_full[h]), 1);
-      mbar_init(smem_u32(&ctl.o_free[h]), kRows);
-      mbar_init(smem_u32(&ctl.clean[h]), 2 * kRows);
+      mbar_init(smem_u32(&ctl.o_free[h]), 4);
+      mbar_init(smem_u32(&ctl.clean[h]), 8);
       mbar_init(smem_u32(&ctl.done[h]), 1);
     }
     ctl.abort = 0;
@@ -335,30 +335,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(smem_u32(&ctl.full[stage_of(i)]), phase_of(i), nullptr);
       }
     }
-  } else if (warp > 8) {
+  } else if (warp < 11) {
     // ------------------------------------------------------------------------------------- MMA
     const int half = warp - 9;
-    if (lane == 0 && half < 2) {
-      const uint32_t s_tmem = tmem + half * 128;
-      const uint32_t o_tmem = tmem + kTmemO + half * 128;
-      const uint32_t q_at = q_smem + half * kOperand;
-      uint32_t turn = 0;  // blocks so far
-      uint32_t segment = 0;
-      uint32_t cleaned[2] = {0, 0};
-      do {
-        int h_begin, h_end;
-        w.half_range(half, half_tokens, window, h_begin, h_end);
-        const int end = w.block + w.count;
-        ok = mbar_wait(smem_u32(&ctl.q_full), segment & 1, &ctl.abort);
-        if (!ok) break;
-        // K of block b: S = Q K^T when the half needs it; the stage is released either way
-        auto do_scores = [&](int b, uint32_t n) {
-          const uint32_t stage = stage_of(2 * n);
-          const bool needed = b >= h_begin && b < h_end;
-          // also without need: a release before the fill would count for the stage's use before
-          if (!mbar_wait(smem_u32(&ctl.full[stage]), phase_of(2 * n), &ctl.abort)) return false;
+    const uint32_t s_tmem = tmem + half * 128;
+    const uint32_t o_tmem = tmem + kTmemO + half * 128;
+    const uint32_t q_at = q_smem + half * kOperand;
+    uint32_t turn = 0;  // blocks so far
+    uint32_t segment = 0;
+    uint32_t cleaned[2] = {0, 0};
+    do {
+      int h_begin, h_end;
+      w.half_range(half, half_tokens, window, h_begin, h_end);
+      const int end = w.block + w.count;
+      ok = mbar_wait(smem_u32(&ctl.q_full), segment & 1, &ctl.abort);
+      if (!ok) break;
+      // K of block b: S = Q K^T when the half needs it; the stage is released either way
+      auto do_scores = [&](int b, uint32_t n) {
+        const uint32_t stage = stage_of(2 * n);
+        const bool needed = b >= h_begin && b < h_end;
+        // also without need: a release before the fill would count for the stage's use before
+        if (!mbar_wait(smem_u32(&ctl.full[stage]), phase_of(2 * n), &ctl.abort)) return false;
+        fence_after();
+        if (elect_one()) {
           if (needed) {
-            fence_after();
             const uint32_t k_at = ring + stage * kOperand;
 #pragma unroll
             for (int k = 0; k < kDim / 16; ++k) {
@@ -373,67 +373,74 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           // Q has been read for the last time by this half
           if (needed ? b == h_end - 1 : (h_begin == h_end && b == end - 1)) mma_commit(smem_u32(&ctl.q_empty));
-          return true;
-        };
-        ok = do_scores(w.block, turn);
+        }
+        __syncwarp();
+        return true;
+      };
+      ok = do_scores(w.block, turn);
+      if (!ok) break;
+      bool waited_o = segment == 0;
+      for (int b = w.block; b < end; ++b, ++turn) {
+        const uint32_t v_item = 2 * turn + 1;
+        const uint32_t stage = stage_of(v_item);
+        const bool needed = b >= h_begin && b < h_end;
+        const bool whole = w.whole(b, window);
+        if (needed && !waited_o) {  // the last segment's O has been read
+          ok = mbar_wait(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
+          waited_o = true;
+        }
+        ok = ok && mbar_wait(smem_u32(&ctl.full[stage]), phase_of(v_item), &ctl.abort);
+        if (ok && !whole) {  // V of this block is cleared by the softmax warps first
+          ok = mbar_wait(smem_u32(&ctl.clean[turn & 1]), cleaned[turn & 1] & 1, &ctl.abort);
+          ++cleaned[turn & 1];
+        }
         if (!ok) break;
-        bool waited_o = segment == 0;
-        for (int b = w.block; b < end; ++b, ++turn) {
-          const uint32_t v_item = 2 * turn + 1;
-          const uint32_t stage = stage_of(v_item);
-          const bool needed = b >= h_begin && b < h_end;
-          const bool whole = w.whole(b, window);
-          if (needed && !waited_o) {  // the last segment's O has been read
-            ok = mbar_wait(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
-            waited_o = true;
-          }
-          ok = ok && mbar_wait(smem_u32(&ctl.full[stage]), phase_of(v_item), &ctl.abort);
-          if (ok && !whole) {  // V of this block is cleared by the softmax warps first
-            ok = mbar_wait(smem_u32(&ctl.clean[turn & 1]), cleaned[turn & 1] & 1, &ctl.abort);
-            ++cleaned[turn & 1];
-          }
-          if (!ok) break;
-          const uint32_t v_at = ring + stage * kOperand;
+        const uint32_t v_at = ring + stage * kOperand;
 #pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            ok = ok && mbar_wait(smem_u32(&ctl.p_full[half][part]), turn & 1, &ctl.abort);
-            if (ok && needed) {
-              fence_after();
+        for (int part = 0; part < 2; ++part) {
+          ok = ok && mbar_wait(smem_u32(&ctl.p_full[half][part]), turn & 1, &ctl.abort);
+          fence_after();
+          if (ok && elect_one()) {
+            if (needed) {
 #pragma unroll
               for (int k = part * 4; k < part * 4 + 4; ++k) {
                 mma_ts(o_tmem, s_tmem + k * 8, desc_mn_major(v_at + k * 16 * 128, kHalfBytes), c.idesc_o,
                        (b > h_begin || k > 0) ? 1u : 0u);
               }
             }
+            if (part == 1) {
+              if (needed) {
+                mma_commit(smem_u32(&ctl.empty[stage]));
+                mma_commit(smem_u32(&ctl.o_full[half]));
+              } else {
+                mbar_arrive(smem_u32(&ctl.empty[stage]));
+              }
+            }
           }
-          if (!ok) break;
-          if (needed) {
-            mma_commit(smem_u32(&ctl.empty[stage]));
-            mma_commit(smem_u32(&ctl.o_full[half]));
-          } else {
-            mbar_arrive(smem_u32(&ctl.empty[stage]));
-          }
-          if (b + 1 < end) ok = do_scores(b + 1, turn + 1);
-          if (!ok) break;
+          __syncwarp();
         }
         if (!ok) break;
-        if (!waited_o) {
-          ok = mbar_wait(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
-          if (!ok) break;
-        }
-        // a half without blocks takes part too, so that its softmax warps stay within a segment of it
-        if (h_begin == h_end) mbar_arrive(smem_u32(&ctl.o_full[half]));
-        ++segment;
-      } while (walk_next(w, c));
-      if (!ok) {
-        report_status(a.status, kStatusWaitTimeout);
-        ctl.abort = 1;
+        if (b + 1 < end) ok = do_scores(b + 1, turn + 1);
+        if (!ok) break;
       }
-      // every MMA of this thread has completed before TMEM and shared memory are released
-      mma_commit(smem_u32(&ctl.done[half]));
-      mbar_wait(smem_u32(&ctl.done[half]), 0, nullptr);
+      if (!ok) break;
+      if (!waited_o) {
+        ok = mbar_wait(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
+        if (!ok) break;
+      }
+      // a half without blocks takes part too, so that its softmax warps stay within a segment of it
+      if (h_begin == h_end && lane == 0) mbar_arrive(smem_u32(&ctl.o_full[half]));
+      __syncwarp();
+      ++segment;
+    } while (walk_next(w, c));
+    if (!ok && lane == 0) {
+      report_status(a.status, kStatusWaitTimeout);
+      ctl.abort = 1;
     }
+    // every MMA of this warp has completed before TMEM and shared memory are released
     __syncwarp();
+    if (elect_one()) mma_commit(smem_u32(&ctl.done[half]));
+    mbar_wait(smem_u32(&ctl.done[half]), 0, nullptr);
   }
   } else {
     // --------------------------------------------------------------------------------- softmax
@@ -499,13 +506,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (bad) atomicOr(&ctl.poison, 1u << (segment & 31));
           fence_async_shared();
-          mbar_arrive(smem_u32(&ctl.clean[turn & 1]));
-          ++cleaned[turn & 1];
           __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&ctl.clean[turn & 1]));
+          __syncwarp();
+          ++cleaned[turn & 1];
         }
         if (!needed) {
-          mbar_arrive(smem_u32(&ctl.p_full[half][0]));
-          mbar_arrive(smem_u32(&ctl.p_full[half][1]));
+          if (lane == 0) {
+            mbar_arrive(smem_u32(&ctl.p_full[half][0]));
+            mbar_arrive(smem_u32(&ctl.p_full[half][1]));
+          }
+          __syncwarp();
           continue;
         }
         fence_after();
@@ -578,7 +589,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_st32(s_tmem + part * 32, packed);
           tmem_wait_st();
           fence_before();
-          mbar_arrive(smem_u32(&ctl.p_full[half][part]));
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&ctl.p_full[half][part]));
+          __syncwarp();
         }
 #pragma unroll
         for (int i = 0; i < kChains / 2; ++i) {
@@ -653,9 +666,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      __syncwarp();
       fence_before();
-      mbar_arrive(smem_u32(&ctl.o_free[half]));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&ctl.o_free[half]));
       if (row_in) {
         if (!complete) {
           partials.stats[slot_row] = make_float2(reference, l);
