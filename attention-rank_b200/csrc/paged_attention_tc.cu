@@ -7,7 +7,7 @@
 // One persistent CTA an SM, 384 threads:
 //   warps 0-3, 4-7  softmax of half 0 / 1: thread r owns row r (TMEM lane r) of its half
 //   warp 8          TMA: Q of both halves, K and V blocks into a ring of four stages
-//   warps 9, 10     tcgen05.mma of half 0 / 1 (warp 11 only fills up the warpgroup)
+//   warp 9          tcgen05.mma of both halves (warps 10 and 11 only fill up the warpgroup)
 // TMEM: S0 | S1 | O0 | O1, 128 columns each; P (16-bit) overwrites its S. Per half and block:
 //   S = Q K^T;  softmax warps read S, write P in two halves of 64 keys;  O += P V starts with the first
 //   while the second is being computed;  the next S follows behind it.
@@ -51,6 +51,7 @@ constexpr uint32_t kTmemO = 256;
 constexpr int kJoinThreads = 256;
 constexpr int kJoinRows = 32;                       // rows of a tile that one joining CTA takes
 constexpr float kRescaleThreshold = 8.0f;           // log2 units
+constexpr int kFmaPairs = 0;                        // of 8 pairs of exponentials, those on the FMA pipe
 constexpr int kChains = 4;                          // independent accumulators per row reduction
 
 struct __align__(16) Control {
@@ -63,7 +64,7 @@ struct __align__(16) Control {
   uint64_t o_full[2];
   uint64_t o_free[2];
   uint64_t clean[2];
-  uint64_t done[2];
+  uint64_t done;
   uint32_t tmem_base;
   volatile int abort;
   unsigned poison;  // bit segment % 32: V held a value that is not finite where some row may not look
@@ -210,10 +211,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (tid == 0) {
     mbar_init(smem_u32(&ctl.q_full), 1);
-    mbar_init(smem_u32(&ctl.q_empty), 2);
+    mbar_init(smem_u32(&ctl.q_empty), 1);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(smem_u32(&ctl.full[i]), 1);
-      mbar_init(smem_u32(&ctl.empty[i]), 2);
+      mbar_init(smem_u32(&ctl.empty[i]), 1);
     }
     for (int h = 0; h < 2; ++h) {
       mbar_init(smem_u32(&ctl.s_full[h]), 1);
@@ -222,8 +223,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&ctl.o_full[h]), 1);
       mbar_init(smem_u32(&ctl.o_free[h]), 4);
       mbar_init(smem_u32(&ctl.clean[h]), 8);
-      mbar_init(smem_u32(&ctl.done[h]), 1);
     }
+    mbar_init(smem_u32(&ctl.done), 1);
     ctl.abort = 0;
     ctl.poison = 0;
     mbar_init_fence();
@@ -335,112 +336,109 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(smem_u32(&ctl.full[stage_of(i)]), phase_of(i), nullptr);
       }
     }
-  } else if (warp < 11) {
+  } else if (warp == 9) {
     // ------------------------------------------------------------------------------------- MMA
-    const int half = warp - 9;
-    const uint32_t s_tmem = tmem + half * 128;
-    const uint32_t o_tmem = tmem + kTmemO + half * 128;
-    const uint32_t q_at = q_smem + half * kOperand;
+    // The halves' products are issued in turn, [O += P V, next S] of half 0, then of half 1, which keeps
+    // the halves half a block apart: with a warp for each half they fell into step, their exponentials
+    // sharing the SFU and their products the tensor pipe (985 against 735 us for two 4K chunks).
     uint32_t turn = 0;  // blocks so far
     uint32_t segment = 0;
     uint32_t cleaned[2] = {0, 0};
     do {
-      int h_begin, h_end;
-      w.half_range(half, half_tokens, window, h_begin, h_end);
+      int h_begin[2], h_end[2];
+      w.half_range(0, half_tokens, window, h_begin[0], h_end[0]);
+      w.half_range(1, half_tokens, window, h_begin[1], h_end[1]);
       const int end = w.block + w.count;
-      ok = mbar_wait(smem_u32(&ctl.q_full), segment & 1, &ctl.abort);
-      if (!ok) break;
-      // K of block b: S = Q K^T when the half needs it; the stage is released either way
-      auto do_scores = [&](int b, uint32_t n) {
-        const uint32_t stage = stage_of(2 * n);
-        const bool needed = b >= h_begin && b < h_end;
-        // also without need: a release before the fill would count for the stage's use before
-        if (!mbar_wait(smem_u32(&ctl.full[stage]), phase_of(2 * n), &ctl.abort)) return false;
-        fence_after();
+      // S = Q K^T of block b (the n-th of the part) where the half needs it
+      auto scores = [&](int half, int b, uint32_t n) {
         if (elect_one()) {
-          if (needed) {
-            const uint32_t k_at = ring + stage * kOperand;
+          if (b >= h_begin[half] && b < h_end[half]) {
+            const uint32_t q_at = q_smem + half * kOperand;
+            const uint32_t k_at = ring + stage_of(2 * n) * kOperand;
 #pragma unroll
             for (int k = 0; k < kDim / 16; ++k) {
               const uint32_t offset = (k >> 2) * kHalfBytes + (k & 3) * 32;
-              mma_ss(s_tmem, desc_k_major(q_at + offset), desc_k_major(k_at + offset), c.idesc_s, k > 0 ? 1u : 0u);
+              mma_ss(tmem + half * 128, desc_k_major(q_at + offset), desc_k_major(k_at + offset), c.idesc_s,
+                     k > 0 ? 1u : 0u);
             }
             mma_commit(smem_u32(&ctl.s_full[half]));
-            mma_commit(smem_u32(&ctl.empty[stage]));
           } else {
             mbar_arrive(smem_u32(&ctl.s_full[half]));
-            mbar_arrive(smem_u32(&ctl.empty[stage]));
           }
-          // Q has been read for the last time by this half
-          if (needed ? b == h_end - 1 : (h_begin == h_end && b == end - 1)) mma_commit(smem_u32(&ctl.q_empty));
+          if (half == 1) {
+            mma_commit(smem_u32(&ctl.empty[stage_of(2 * n)]));
+            if (b == end - 1) mma_commit(smem_u32(&ctl.q_empty));  // Q has been read for the last time
+          }
         }
         __syncwarp();
-        return true;
       };
-      ok = do_scores(w.block, turn);
+      auto wait_k = [&](uint32_t n) {
+        const bool there = mbar_wait(smem_u32(&ctl.full[stage_of(2 * n)]), phase_of(2 * n), &ctl.abort);
+        fence_after();
+        return there;
+      };
+      ok = mbar_wait(smem_u32(&ctl.q_full), segment & 1, &ctl.abort) && wait_k(turn);
       if (!ok) break;
-      bool waited_o = segment == 0;
-      for (int b = w.block; b < end; ++b, ++turn) {
+      scores(0, w.block, turn);
+      scores(1, w.block, turn);
+      bool waited_o[2] = {segment == 0, segment == 0};
+      for (int b = w.block; ok && b < end; ++b, ++turn) {
         const uint32_t v_item = 2 * turn + 1;
         const uint32_t stage = stage_of(v_item);
-        const bool needed = b >= h_begin && b < h_end;
-        const bool whole = w.whole(b, window);
-        if (needed && !waited_o) {  // the last segment's O has been read
-          ok = mbar_wait(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
-          waited_o = true;
-        }
-        ok = ok && mbar_wait(smem_u32(&ctl.full[stage]), phase_of(v_item), &ctl.abort);
-        if (ok && !whole) {  // V of this block is cleared by the softmax warps first
+        ok = mbar_wait(smem_u32(&ctl.full[stage]), phase_of(v_item), &ctl.abort);
+        if (ok && !w.whole(b, window)) {  // V of this block is cleared by the softmax warps first
           ok = mbar_wait(smem_u32(&ctl.clean[turn & 1]), cleaned[turn & 1] & 1, &ctl.abort);
           ++cleaned[turn & 1];
         }
-        if (!ok) break;
         const uint32_t v_at = ring + stage * kOperand;
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          ok = ok && mbar_wait(smem_u32(&ctl.p_full[half][part]), turn & 1, &ctl.abort);
-          fence_after();
-          if (ok && elect_one()) {
-            if (needed) {
-#pragma unroll
-              for (int k = part * 4; k < part * 4 + 4; ++k) {
-                mma_ts(o_tmem, s_tmem + k * 8, desc_mn_major(v_at + k * 16 * 128, kHalfBytes), c.idesc_o,
-                       (b > h_begin || k > 0) ? 1u : 0u);
-              }
-            }
-            if (part == 1) {
-              if (needed) {
-                mma_commit(smem_u32(&ctl.empty[stage]));
-                mma_commit(smem_u32(&ctl.o_full[half]));
-              } else {
-                mbar_arrive(smem_u32(&ctl.empty[stage]));
-              }
-            }
+        for (int half = 0; half < 2; ++half) {
+          const bool needed = b >= h_begin[half] && b < h_end[half];
+          if (ok && needed && !waited_o[half]) {  // the last segment's O has been read
+            ok = mbar_wait(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
+            waited_o[half] = true;
           }
-          __syncwarp();
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            ok = ok && mbar_wait(smem_u32(&ctl.p_full[half][part]), turn & 1, &ctl.abort);
+            fence_after();
+            if (ok && elect_one()) {
+              if (needed) {
+#pragma unroll
+                for (int k = part * 4; k < part * 4 + 4; ++k) {
+                  mma_ts(tmem + kTmemO + half * 128, tmem + half * 128 + k * 8,
+                         desc_mn_major(v_at + k * 16 * 128, kHalfBytes), c.idesc_o,
+                         (b > h_begin[half] || k > 0) ? 1u : 0u);
+                }
+                if (part == 1) mma_commit(smem_u32(&ctl.o_full[half]));
+              }
+              if (half == 1 && part == 1) mma_commit(smem_u32(&ctl.empty[stage]));
+            }
+            __syncwarp();
+          }
+          if (ok && b + 1 < end) {
+            if (half == 0) ok = wait_k(turn + 1);
+            if (ok) scores(half, b + 1, turn + 1);
+          }
         }
-        if (!ok) break;
-        if (b + 1 < end) ok = do_scores(b + 1, turn + 1);
-        if (!ok) break;
       }
-      if (!ok) break;
-      if (!waited_o) {
-        ok = mbar_wait(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
-        if (!ok) break;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (ok && !waited_o[half]) ok = mbar_wait(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
+        // a half without blocks takes part too, so that its softmax warps stay within a segment of it
+        if (ok && h_begin[half] == h_end[half] && lane == 0) mbar_arrive(smem_u32(&ctl.o_full[half]));
+        __syncwarp();
       }
-      // a half without blocks takes part too, so that its softmax warps stay within a segment of it
-      if (h_begin == h_end && lane == 0) mbar_arrive(smem_u32(&ctl.o_full[half]));
-      __syncwarp();
       ++segment;
-    } while (walk_next(w, c));
+    } while (ok && walk_next(w, c));
     if (!ok && lane == 0) {
       report_status(a.status, kStatusWaitTimeout);
       ctl.abort = 1;
     }
-    // every MMA of this warp has completed before TMEM and shared memory are released
+    // every MMA has completed before TMEM and shared memory are released
     __syncwarp();
-    if (elect_one()) mma_commit(smem_u32(&ctl.done[half]));
-    mbar_wait(smem_u32(&ctl.done[half]), 0, nullptr);
+    if (elect_one()) mma_commit(smem_u32(&ctl.done));
+    mbar_wait(smem_u32(&ctl.done), 0, nullptr);
   }
   } else {
     // --------------------------------------------------------------------------------- softmax
@@ -542,9 +540,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < kChains; ++i) top[i] = x[i];
 #pragma unroll
         for (int i = kChains; i < kChunkBlock; i += 2) {
-          top[(i / 2) % kChains] = max3(top[(i / 2) % kChains], x[i], x[i + 1]);
+          top[(i / 2) % kChains] = max3_nan(top[(i / 2) % kChains], x[i], x[i + 1]);
         }
-        const float block_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+        const float block_top = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
         // the row's reference moves only when the block's maximum exceeds it by more than the threshold,
         // so probabilities stay below 2^8 and O is rarely rescaled
         const bool move = block_top > reference + kRescaleThreshold || (reference == -INFINITY && block_top != -INFINITY);
@@ -573,25 +571,62 @@ __global__ void __launch_bounds__(kThreads, 1)
         unsigned long long sums[kChains / 2];
 #pragma unroll
         for (int i = 0; i < kChains / 2; ++i) sums[i] = 0ull;
+        // Groups of eight pairs, of which kFmaPairs run on the FMA pipe (where every score is finite): the
+        // SFU's are issued first, its results are used a group later.
+        auto probabilities = [&](auto share) {
+          constexpr int kFma = decltype(share)::value;
+          constexpr int kSfu = 8 - kFma;
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          uint32_t packed[32];
+          for (int part = 0; part < 2; ++part) {
+            uint32_t packed[32];
+            float p[2][16];
+            auto finish = [&](int group) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int at = part * 64 + 2 * i;
-            float t0, t1;
-            unpack_f32x2(fma_f32x2(pack_f32x2(x[at], x[at + 1]), scale2, base2), t0, t1);
-            const float p0 = ex2_ftz(t0);
-            const float p1 = ex2_ftz(t1);
-            sums[i % (kChains / 2)] = add_f32x2(sums[i % (kChains / 2)], pack_f32x2(p0, p1));
-            packed[i] = pack2<T>(p0, p1);
+              for (int i = 0; i < 8; ++i) {
+                const float p0 = p[group & 1][2 * i], p1 = p[group & 1][2 * i + 1];
+                sums[i % (kChains / 2)] = add_f32x2(sums[i % (kChains / 2)], pack_f32x2(p0, p1));
+                packed[group * 8 + i] = pack2<T>(p0, p1);
+              }
+            };
+#pragma unroll
+            for (int group = 0; group < 4; ++group) {
+              unsigned long long t[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int at = part * 64 + group * 16 + 2 * i;
+                t[i] = fma_f32x2(pack_f32x2(x[at], x[at + 1]), scale2, base2);
+              }
+#pragma unroll
+              for (int i = 0; i < kSfu; ++i) {
+                float t0, t1;
+                unpack_f32x2(t[i], t0, t1);
+                p[group & 1][2 * i] = ex2_ftz(t0);
+                p[group & 1][2 * i + 1] = ex2_ftz(t1);
+              }
+              if constexpr (kFma > 0) {
+                unsigned long long rest[kFma];
+                float out[2 * kFma];
+#pragma unroll
+                for (int i = 0; i < kFma; ++i) rest[i] = t[kSfu + i];
+                exp2_fma<kFma>(rest, out);
+#pragma unroll
+                for (int i = 0; i < 2 * kFma; ++i) p[group & 1][2 * kSfu + i] = out[i];
+              }
+              if (group > 0) finish(group - 1);
+            }
+            finish(3);
+            tmem_st32(s_tmem + part * 32, packed);
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&ctl.p_full[half][part]));
+            __syncwarp();
           }
-          tmem_st32(s_tmem + part * 32, packed);
-          tmem_wait_st();
-          fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&ctl.p_full[half][part]));
-          __syncwarp();
+        };
+        if (whole && __all_sync(0xffffffffu, !row_in || fabsf(block_top) < INFINITY)) {
+          probabilities(std::integral_constant<int, kFmaPairs>{});
+        } else {
+          probabilities(std::integral_constant<int, 0>{});
         }
 #pragma unroll
         for (int i = 0; i < kChains / 2; ++i) {
@@ -621,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool complete = begins && w.count == w.tile.blocks;
       const float factor = complete ? (l != 0.0f ? 1.0f / l : 0.0f) : 1.0f;
       const int head = w.kv_head * group + row_head;
-      const int64_t slot_row = (static_cast<int64_t>(blockIdx.x) * 2 + (begins ? 1 : 0)) * (2 * kRows) + half * kRows + row;
+      const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (begins ? 1 : 0);
       const int64_t out_token = w.seq.q_begin + token;
 #pragma unroll 1
       for (int i = 0; i < kDim / 32; ++i) {
@@ -652,16 +687,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < 16; ++j) {
             packed[j] = pack2<T>(__uint_as_float(raw[2 * j]) * factor, __uint_as_float(raw[2 * j + 1]) * factor);
           }
-          uint4* to16 = reinterpret_cast<uint4*>(to);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            to16[j] = make_uint4(packed[4 * j], packed[4 * j + 1], packed[4 * j + 2], packed[4 * j + 3]);
-          }
+          *reinterpret_cast<uint4*>(to) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+          *reinterpret_cast<uint4*>(to + 8) = make_uint4(packed[4], packed[5], packed[6], packed[7]);
+          *reinterpret_cast<uint4*>(to + 16) = make_uint4(packed[8], packed[9], packed[10], packed[11]);
+          *reinterpret_cast<uint4*>(to + 24) = make_uint4(packed[12], packed[13], packed[14], packed[15]);
         } else if (row_in) {
-          float4* to = reinterpret_cast<float4*>(partials.sums + slot_row * kDim + i * 32);
+          // [columns / 4][rows][4]: a warp's rows are neighbours
+          float4* to = reinterpret_cast<float4*>(partials.sums) + slot * (2 * kRows) * (kDim / 4) +
+                       i * 8 * (2 * kRows) + half * kRows + row;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            to[j] = make_float4(__uint_as_float(raw[4 * j]), __uint_as_float(raw[4 * j + 1]),
+            to[j * (2 * kRows)] = make_float4(__uint_as_float(raw[4 * j]), __uint_as_float(raw[4 * j + 1]),
                                 __uint_as_float(raw[4 * j + 2]), __uint_as_float(raw[4 * j + 3]));
           }
         }
@@ -671,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(smem_u32(&ctl.o_free[half]));
       if (row_in) {
         if (!complete) {
-          partials.stats[slot_row] = make_float2(reference, l);
+          partials.stats[slot * (2 * kRows) + half * kRows + row] = make_float2(reference, l);
         } else if (a.lse != nullptr) {
           a.lse[out_token * a.query_heads + head] = l != 0.0f ? reference + log2f(l) : -INFINITY;
         }
@@ -721,55 +757,57 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_chunk_join_kerne
   const int group = a.query_heads / a.cache.kv_heads;
   const PartialSums<2 * kRows, kDim> partials(a.workspace, ctas);
   constexpr int kBatch = 4;  // parts whose loads are in flight together
-  for (int item = threadIdx.x; item < kJoinRows * (kDim / 4); item += kJoinThreads) {
-    const int tile_row = blockIdx.y * kJoinRows + item / (kDim / 4);
-    const int column = item % (kDim / 4) * 4;
-    const int half = tile_row / kRows;
-    const int row = tile_row - half * kRows;
-    const int row_token = row / group;
-    const int token = (place.t * 2 + half) * c.half_tokens + row_token;
-    if (row_token >= c.half_tokens || token >= seq.q_len) continue;
+  // a warp takes 32 rows of eight columns
+  const int tile_row = blockIdx.y * kJoinRows + (threadIdx.x & 31);
+  const int half = tile_row / kRows;
+  const int row = tile_row - half * kRows;
+  const int row_token = row / group;
+  const int token = (place.t * 2 + half) * c.half_tokens + row_token;
+  if (row_token >= c.half_tokens || token >= seq.q_len) return;
+  const int head = place.kv_head * group + row - row_token * group;
+  for (int column = (threadIdx.x >> 5) * 8; column < kDim; column += kJoinThreads / 32 * 8) {
     float top = -INFINITY;
     float sum = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float o[8] = {};
     for (int first = boundary; first <= last; first += kBatch) {
       float2 stats[kBatch];
-      float4 piece[kBatch];
+      float4 piece[kBatch][2];
       float high = top;
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const int part = first + i;
         stats[i] = make_float2(-INFINITY, 0.0f);
-        piece[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        piece[i][0] = piece[i][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (part <= last) {
-          const int64_t at_row = (static_cast<int64_t>(part) * 2 + (part == boundary ? 1 : 0)) * (2 * kRows) + tile_row;
-          stats[i] = partials.stats[at_row];
-          piece[i] = *reinterpret_cast<const float4*>(partials.sums + at_row * kDim + column);
+          const int64_t slot = static_cast<int64_t>(part) * 2 + (part == boundary ? 1 : 0);
+          const float4* from = reinterpret_cast<const float4*>(partials.sums) + slot * (2 * kRows) * (kDim / 4) +
+                               column / 4 * (2 * kRows) + tile_row;
+          stats[i] = partials.stats[slot * (2 * kRows) + tile_row];
+          piece[i][0] = from[0];
+          piece[i][1] = from[2 * kRows];
         }
         high = fmaxf(high, stats[i].x);
       }
       const float keep = top == -INFINITY ? 0.0f : ex2_ftz(top - high);
       sum *= keep;
-      o.x *= keep;
-      o.y *= keep;
-      o.z *= keep;
-      o.w *= keep;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] *= keep;
       top = high;
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const float factor = stats[i].x == -INFINITY ? 0.0f : ex2_ftz(stats[i].x - top);
         sum += factor * stats[i].y;
-        o.x += factor * piece[i].x;
-        o.y += factor * piece[i].y;
-        o.z += factor * piece[i].z;
-        o.w += factor * piece[i].w;
+        const float values[8] = {piece[i][0].x, piece[i][0].y, piece[i][0].z, piece[i][0].w,
+                                 piece[i][1].x, piece[i][1].y, piece[i][1].z, piece[i][1].w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] += factor * values[j];
       }
     }
     const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
-    const int head = place.kv_head * group + row - row_token * group;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] *= inverse;
     T* to = static_cast<T*>(a.out) + (seq.q_begin + token) * a.out_stride + head * kDim + column;
-    *reinterpret_cast<uint2*>(to) =
-        make_uint2(pack2<T>(o.x * inverse, o.y * inverse), pack2<T>(o.z * inverse, o.w * inverse));
+    *reinterpret_cast<uint4*>(to) = pack8<T>(o);
     if (column == 0 && a.lse != nullptr) {
       a.lse[static_cast<int64_t>(seq.q_begin + token) * a.query_heads + head] =
           sum != 0.0f ? top + log2f(sum) : -INFINITY;
