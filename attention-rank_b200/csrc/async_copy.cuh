@@ -83,6 +83,24 @@ __device__ __forceinline__ float ex2_ftz(float x) {
 
 }  // namespace async
 
+// Launches with programmatic stream serialization: the kernel may start while the one before it on the
+// stream ends, and every thread of it calls wait_for_producer() before it reads or writes memory.
+template <typename... Parameters, typename... Arguments>
+cudaError_t launch_overlapped(void (*kernel)(Parameters...), dim3 grid, dim3 block, size_t shared, cudaStream_t stream,
+                              Arguments... arguments) {
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.dynamicSmemBytes = shared;
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, arguments...);
+}
+
 inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;

@@ -102,7 +102,8 @@ int64_t paged_attention_workspace(const PagedCache& cache, const PagedBatch& bat
 cudaError_t launch_paged_attention(const PagedAttentionArgs& args, cudaStream_t stream);
 // The form for more than a few rows a KV head (paged_attention_tc.cu).
 int64_t paged_attention_chunk_workspace(int head_dim);
-cudaError_t launch_paged_attention_chunk(const PagedAttentionArgs& args, cudaStream_t stream);
+// It leaves out sequences of at most `few` new tokens.
+cudaError_t launch_paged_attention_chunk(const PagedAttentionArgs& args, int few, cudaStream_t stream);
 
 // ------------------------------------------------------------------------------ device helpers
 #ifdef __CUDACC__

@@ -52,10 +52,9 @@ __device__ __forceinline__ FewTile few_tile(const PagedSequence& seq, int window
   return t;
 }
 
-// Units of sequence s (0 without new tokens).
-__device__ __forceinline__ int64_t few_units(const PagedAttentionArgs& a, int s) {
-  const PagedSequence seq = paged_sequence(a.batch, s, a.status);
-  if (seq.q_len == 0) return 0;
+// Units of a sequence; 0 without new tokens, or with more of them than this form takes.
+__device__ __forceinline__ int64_t few_units(const PagedAttentionArgs& a, const PagedSequence& seq, int most) {
+  if (seq.q_len == 0 || seq.q_len > most) return 0;
   return static_cast<int64_t>(few_tile(seq, a.sliding_window).blocks) * a.cache.kv_heads;
 }
 
@@ -153,7 +152,7 @@ __device__ float nonfinite_sum(const PagedAttentionArgs& a, int s, int kv_head, 
 template <typename T, int kGroups, int kDim>
 __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<kGroups, kDim>::kCtasPerSm)
     paged_attention_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                               const PagedAttentionArgs a) {
+                               const PagedAttentionArgs a, int most) {
   using Shared = FewShared<kGroups, kDim>;
   constexpr int kThreads = Shared::kThreads;
   constexpr int kStages = Shared::kStages;
@@ -178,29 +177,34 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
     prefetch_map(&k_map);
     prefetch_map(&v_map);
   }
-  const int64_t total = plan_total<kThreads>(a.batch.sequences, sh.plan, [&](int s) { return few_units(a, s); });  // its barriers cover the set-up above
-  const int parts = plan_parts(total, gridDim.x);
+  wait_for_producer();
   release_dependents();  // the joining kernel waits for this one's completion by itself
-  if (blockIdx.x >= parts) return;
-  const int64_t begin = part_begin(total, blockIdx.x, parts);
-  const int64_t end = part_begin(total, blockIdx.x + 1, parts);
-  const PlanPlace place =
-      plan_locate<kThreads>(a.batch.sequences, begin, sh.plan, [&](int s) { return few_units(a, s); });
+  const PartialSums<kRows, kDim> partials(a.workspace, gridDim.x);
+  PlanPlace place;  // the barriers inside also cover the set-up above
+  const bool has_part = plan_part<kThreads>(
+      a.batch, a.status, gridDim.x, sh.plan,
+      [&](const PagedSequence& seq) { return few_units(a, seq, most); }, place);
+  if (!has_part) {
+    if (tid == 0) leave_join_tile(partials.tiles, nullptr, 0, 0, 0, 0);
+    return;
+  }
 
   // walk of the part, the same for every role: segments of one (sequence, KV head)
   int s = place.sequence;
-  PagedSequence seq = paged_sequence(a.batch, s, nullptr);
+  PagedSequence seq = place.seq;
   FewTile tile = few_tile(seq, a.sliding_window);
-  int kv_head = static_cast<int>((begin - place.before) / tile.blocks);
+  const int64_t begin = place.cut.begin(blockIdx.x);
+  int kv_head = static_cast<int>(PlanCut::divide(begin - place.before, tile.blocks));
   int block = static_cast<int>(begin - place.before - static_cast<int64_t>(kv_head) * tile.blocks);
-  int64_t left = end - begin;
+  int64_t left = place.cut.begin(blockIdx.x + 1) - begin;
+  if (tid == 0) leave_join_tile(partials.tiles, &place, 0, kv_head, begin - block, tile.blocks);
   auto next_tile = [&] {
     block = 0;
     if (++kv_head < a.cache.kv_heads) return;
     kv_head = 0;
     do {  // `left` units remain, so a sequence with new tokens follows
       seq = paged_sequence(a.batch, ++s, nullptr);
-    } while (seq.q_len == 0 && s + 1 < a.batch.sequences);
+    } while (few_units(a, seq, most) == 0 && s + 1 < a.batch.sequences);
     tile = few_tile(seq, a.sliding_window);
   };
 
@@ -308,20 +312,11 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
     float reference[2] = {-INFINITY, -INFINITY};
     float l[2] = {0.0f, 0.0f};
     bool poison = false;
-    for (int i = 0; i < count; ++i, ++turn) {
-      const int stage = turn % kStages;
-      const bool ready = mbar_wait(smem_u32(&sh.full[stage]), (turn / kStages) & 1, &sh.abort);
-      if (!__all_sync(0xffffffffu, ready)) {
-        ok = false;
-        break;
-      }
-      const int key0 = (tile.block_begin + block + i) * kBlock;
-      // does every row see every key of the block?
-      const bool whole = key0 + kBlock - 1 <= tile.first_position &&
-                         (a.sliding_window == 0 || key0 >= seq.kv_len - a.sliding_window);
+    // scores of a block; the next block's are computed ahead of this one's softmax, which hides them
+    auto scores = [&](uint32_t at_turn, float (&x)[2][4]) {
+      const int stage = at_turn % kStages;
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.full[stage]), (at_turn / kStages) & 1, &sh.abort))) return false;
       const uint32_t k_at = k_smem + stage * kBlockBytes + k_row;
-      const uint32_t v_at = v_smem + stage * kBlockBytes + v_row;
-      float x[2][4];
 #pragma unroll
       for (int n = 0; n < 2; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
 #pragma unroll
@@ -331,36 +326,63 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
         mma_16816<T>(x[0], q[k], b[0], b[1]);
         mma_16816<T>(x[1], q[k], b[2], b[3]);
       }
+      return true;
+    };
+    float x[2][4];
+    ok = scores(turn, x);
+    for (int i = 0; ok && i < count; ++i, ++turn) {
+      float following[2][4];
+      if (i + 1 < count) ok = scores(turn + 1, following);
+      if (!ok) break;
+      const int key0 = (tile.block_begin + block + i) * kBlock;
       const int key = key0 + quarter * 16 + 2 * t4;  // of x[0][0]
-      uint32_t p[4];
+      // does every row see every key of the block?
+      const bool whole = key0 + kBlock - 1 <= tile.first_position &&
+                         (a.sliding_window == 0 || key0 >= seq.kv_len - a.sliding_window);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {  // rows g, g + 8
-        float top = -INFINITY;
+      for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[n][c] *= a.scale_log2;
+      }
+      if (!whole) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float& v = x[n][2 * e + c];
-            const int at = key + 8 * n + c;
-            v = whole || (at <= last_key[e] && at >= first_key[e]) ? v * a.scale_log2 : -INFINITY;
-            top = fmaxf(top, v);
+          for (int c = 0; c < 4; ++c) {
+            const int at = key + 8 * n + (c & 1);
+            if (at > last_key[c >> 1] || at < first_key[c >> 1]) x[n][c] = -INFINITY;
           }
         }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the reference moves only when the block's maximum exceeds it by more than the threshold, so
-        // probabilities stay below 2^8 and the sums are rarely rescaled
-        const bool move = top > reference[e] + kRescaleThreshold || (reference[e] == -INFINITY && top != -INFINITY);
-        if (__any_sync(0xffffffffu, move)) {
-          const float factor = move ? (reference[e] == -INFINITY ? 0.0f : ex2_ftz(reference[e] - top)) : 1.0f;
-          if (move) reference[e] = top;
-          l[e] *= factor;
+      }
+      // The reference moves only when a score exceeds it by more than the threshold, so probabilities
+      // stay below 2^8; the row's maximum is only looked for then.
+      float top[2];
+      bool move = false;
 #pragma unroll
-          for (int d = 0; d < kDim / 8; ++d) {
-            o[d][2 * e] *= factor;
-            o[d][2 * e + 1] *= factor;
+      for (int e = 0; e < 2; ++e) {
+        top[e] = fmaxf(fmaxf(x[0][2 * e], x[0][2 * e + 1]), fmaxf(x[1][2 * e], x[1][2 * e + 1]));
+        move |= top[e] > reference[e] + kRescaleThreshold || (reference[e] == -INFINITY && top[e] != -INFINITY);
+      }
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
+          top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
+          if (top[e] > reference[e]) {
+            const float factor = reference[e] == -INFINITY ? 0.0f : ex2_ftz(reference[e] - top[e]);
+            reference[e] = top[e];
+            l[e] *= factor;
+#pragma unroll
+            for (int d = 0; d < kDim / 8; ++d) {
+              o[d][2 * e] *= factor;
+              o[d][2 * e + 1] *= factor;
+            }
           }
         }
+      }
+      uint32_t p[4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
         const float base = reference[e] == -INFINITY ? 0.0f : reference[e];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -370,6 +392,8 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
           p[2 * n + e] = pack2<T>(p0, p1);
         }
       }
+      const int stage = turn % kStages;
+      const uint32_t v_at = v_smem + stage * kBlockBytes + v_row;
 #pragma unroll
       for (int d = 0; d < kDim / 16; ++d) {
         uint32_t b[4];
@@ -385,6 +409,11 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.empty[stage]));
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[n][c] = following[n][c];
+      }
     }
     if (!ok) break;
 
@@ -403,7 +432,6 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
     const bool begins = block == 0;
     const bool complete = begins && count == tile.blocks;
     const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (begins ? 1 : 0);
-    const PartialSums<kRows, kDim> partials(a.workspace, gridDim.x);
     auto joined = [&](int row) {  // (reference, sum) of one of the 16 rows over the warps
       float2 all = make_float2(-INFINITY, 0.0f);
 #pragma unroll
@@ -488,39 +516,24 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
   }
 }
 
-// Joins the parts of the tile that the boundary between CTAs c and c + 1 cuts, for the first such
-// boundary of each tile, in the order of the CTAs.
+// Joins the parts of the tile that the beginning of part blockIdx.x + 1 cuts, in the order of the CTAs.
 template <typename T, int kRows, int kDim>
 __global__ void __launch_bounds__(kCombineThreads) paged_attention_few_join_kernel(const PagedAttentionArgs a, int ctas) {
-  __shared__ PlanScratch<kCombineThreads> plan;
-  const int64_t total =
-      plan_total<kCombineThreads>(a.batch.sequences, plan, [&](int s) { return few_units(a, s); });
-  const int parts = plan_parts(total, ctas);
-  const int c = blockIdx.x;  // the boundary between parts c and c + 1
-  const int64_t at = part_begin(total, c + 1, max(parts, 1));
-  bool cut = c + 1 < parts;
-  PagedSequence seq{};
-  FewTile tile{};
-  int kv_head = 0;
-  int last = 0;  // part that holds the tile's last unit
-  if (cut) {
-    const PlanPlace place =
-        plan_locate<kCombineThreads>(a.batch.sequences, at, plan, [&](int s) { return few_units(a, s); });
-    seq = paged_sequence(a.batch, place.sequence, nullptr);
-    tile = few_tile(seq, a.sliding_window);
-    kv_head = static_cast<int>((at - place.before) / tile.blocks);
-    const int64_t tile_begin = place.before + static_cast<int64_t>(kv_head) * tile.blocks;
-    cut = tile_begin < at && part_begin(total, c, parts) <= tile_begin;
-    last = part_of(total, tile_begin + tile.blocks - 1, parts);
-  }
-  // every CTA waits, so that this grid does not complete before the one whose sums it reads
+  // every thread waits, so that this grid does not complete before the one whose sums it reads
   wait_for_producer();
-  if (!cut) return;
+  release_dependents();
+  const PartialSums<kRows, kDim> partials(a.workspace, ctas);
+  const JoinTile join = partials.tiles[blockIdx.x + 1];
+  const int last = join.last;
+  if (last < 0) return;
+  const PagedSequence seq = join.seq;
+  const int kv_head = join.kv_head;
+  const int c = blockIdx.x;  // the part in which the tile begins
   const int group = a.query_heads / a.cache.kv_heads;
   const int rows = seq.q_len * group;
-  const PartialSums<kRows, kDim> partials(a.workspace, ctas);
   constexpr int kBatch = 8;  // parts whose loads are in flight together
-  for (int item = threadIdx.x; item < rows * (kDim / 4); item += kCombineThreads) {
+  for (int item = blockIdx.y * kCombineThreads + threadIdx.x; item < rows * (kDim / 4);
+       item += gridDim.y * kCombineThreads) {
     const int row = item / (kDim / 4);
     const int column = (item - row * (kDim / 4)) * 4;
     float top = -INFINITY;
@@ -595,8 +608,9 @@ int few_ctas() {
   return sm_count() * FewShared<kGroups, 128>::kCtasPerSm;
 }
 
+// Takes the sequences of at most `most` new tokens.
 template <typename T, int kGroups, int kDim>
-cudaError_t launch_few(const PagedAttentionArgs& a, cudaStream_t stream) {
+cudaError_t launch_few(const PagedAttentionArgs& a, int most, cudaStream_t stream) {
   using Shared = FewShared<kGroups, kDim>;
   static_assert(Shared::kCtasPerSm * (Shared::bytes() + 1024) <= 228 * 1024, "the CTAs of an SM share its shared memory");
   int device = 0;
@@ -616,37 +630,57 @@ cudaError_t launch_few(const PagedAttentionArgs& a, cudaStream_t stream) {
     return cudaErrorInvalidValue;
   }
   const int ctas = few_ctas<kGroups>();
-  paged_attention_few_kernel<T, kGroups, kDim><<<ctas, Shared::kThreads, Shared::bytes(), stream>>>(k_map, v_map, a);
-  cudaError_t status = cudaGetLastError();
-  if (status != cudaSuccess) return status;
-  cudaLaunchAttribute attribute;
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(ctas - 1);
-  config.blockDim = dim3(kCombineThreads);
-  config.stream = stream;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
-  status = cudaLaunchKernelEx(&config, paged_attention_few_join_kernel<T, Shared::kRows, kDim>, a, ctas);
-  return status != cudaSuccess ? status : cudaGetLastError();
+  const cudaError_t status = launch_overlapped(paged_attention_few_kernel<T, kGroups, kDim>, dim3(ctas),
+                                               dim3(Shared::kThreads), Shared::bytes(), stream, k_map, v_map, a, most);
+  if (status != cudaSuccess || ctas < 2) return status;
+  return launch_overlapped(paged_attention_few_join_kernel<T, Shared::kRows, kDim>, dim3(ctas - 1, Shared::kRows / 8),
+                           dim3(kCombineThreads), 0, stream, a, ctas);
+}
+
+// Which forms a batch takes. A sequence's rows are its new tokens times the query heads of a KV head.
+// Where no sequence has more than 32 rows the kernel of this file takes them all. Else the chunk kernel
+// takes them, except that in a batch of several sequences those of at most 16 rows go to this kernel
+// first, which reads the cache at HBM's rate where a 256-row tile of the other would be nearly empty
+// (13 single tokens and 6 chunks: CHOICE_TIMES).
+struct FormChoice {
+  int few_rows = 0;    // 16, 32, or 0: the few-row form is not launched
+  int few_tokens = 0;  // new tokens up to which a sequence takes it
+  bool chunk = false;  // is the chunk form launched?
+};
+
+FormChoice choose_forms(const PagedCache& cache, const PagedBatch& batch, int query_heads) {
+  const int group = query_heads / cache.kv_heads;
+  const int64_t rows = static_cast<int64_t>(batch.max_query) * group;
+  FormChoice choice;
+  choice.chunk = rows > 32;
+  if (!choice.chunk) {
+    choice.few_rows = rows <= 16 ? 16 : 32;
+  } else if (batch.sequences > 1 && group <= 16) {
+    choice.few_rows = 16;
+  }
+  choice.few_tokens = choice.few_rows / group;
+  return choice;
 }
 
 template <typename T, int kDim>
 cudaError_t launch_dim(const PagedAttentionArgs& a, cudaStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(a.batch.max_query) * (a.query_heads / a.cache.kv_heads);
-  if (rows <= 16) return launch_few<T, 1, kDim>(a, stream);
-  if (rows <= 32) return launch_few<T, 2, kDim>(a, stream);
-  return launch_paged_attention_chunk(a, stream);
+  const FormChoice choice = choose_forms(a.cache, a.batch, a.query_heads);
+  cudaError_t status = cudaSuccess;
+  if (choice.few_rows == 16) status = launch_few<T, 1, kDim>(a, choice.few_tokens, stream);
+  if (choice.few_rows == 32) status = launch_few<T, 2, kDim>(a, choice.few_tokens, stream);
+  if (status != cudaSuccess || !choice.chunk) return status;
+  // the two forms' partial sums share the workspace: each kernel waits for the one before it
+  return launch_paged_attention_chunk(a, choice.few_tokens, stream);
 }
 
 }  // namespace
 
 int64_t paged_attention_workspace(const PagedCache& cache, const PagedBatch& batch, int query_heads) {
-  const int64_t rows = static_cast<int64_t>(batch.max_query) * (query_heads / cache.kv_heads);
-  if (rows <= 16) return partial_bytes(16, cache.head_dim, few_ctas<1>());
-  if (rows <= 32) return partial_bytes(32, cache.head_dim, few_ctas<2>());
-  return paged_attention_chunk_workspace(cache.head_dim);
+  const FormChoice choice = choose_forms(cache, batch, query_heads);
+  int64_t bytes = choice.chunk ? paged_attention_chunk_workspace(cache.head_dim) : 0;
+  if (choice.few_rows == 16) bytes = std::max(bytes, partial_bytes(16, cache.head_dim, few_ctas<1>()));
+  if (choice.few_rows == 32) bytes = std::max(bytes, partial_bytes(32, cache.head_dim, few_ctas<2>()));
+  return bytes;
 }
 
 cudaError_t launch_paged_attention(const PagedAttentionArgs& a, cudaStream_t stream) {

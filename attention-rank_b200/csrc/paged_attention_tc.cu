@@ -89,40 +89,15 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
 struct ChunkArgs {
   PagedAttentionArgs a;
   int half_tokens;  // tokens of half a tile
+  int few;          // sequences of at most so many new tokens are left out
   uint32_t idesc_s;
   uint32_t idesc_o;
 };
 
-__device__ __forceinline__ int64_t chunk_units(const ChunkArgs& c, int s) {
-  const PagedSequence seq = paged_sequence(c.a.batch, s, c.a.status);
+// Units of a sequence: the key blocks of all its tiles, for every KV head.
+__device__ __forceinline__ int64_t chunk_units(const ChunkArgs& c, const PagedSequence& seq) {
+  if (seq.q_len <= c.few) return 0;
   return chunk_blocks(seq.q_len, seq.kv_len, 2 * c.half_tokens, c.a.sliding_window) * c.a.cache.kv_heads;
-}
-
-// A place in the line: block `block` of tile `t`, KV head `kv_head`, sequence `s`.
-struct ChunkPlace {
-  int s, t, kv_head, block;
-  int64_t tile_begin;  // the line's unit at which (sequence, tile, KV head) begins
-};
-
-template <int kCount>
-__device__ __forceinline__ ChunkPlace chunk_locate(const ChunkArgs& c, int64_t unit, PlanScratch<kCount>& scratch) {
-  const PlanPlace place = plan_locate<kCount>(c.a.batch.sequences, unit, scratch, [&](int s) { return chunk_units(c, s); });
-  const PagedSequence seq = paged_sequence(c.a.batch, place.sequence, nullptr);
-  const int step = 2 * c.half_tokens;
-  const int tiles = (seq.q_len + step - 1) / step;
-  __syncthreads();  // `place` has been read by everyone
-  const PlanPlace in = plan_locate<kCount>(tiles, unit - place.before, scratch, [&](int t) {
-    return static_cast<int64_t>(chunk_tile(seq.q_len, seq.kv_len, step, c.a.sliding_window, t).blocks) * c.a.cache.kv_heads;
-  });
-  const int blocks = chunk_tile(seq.q_len, seq.kv_len, step, c.a.sliding_window, in.sequence).blocks;
-  const int64_t rest = unit - place.before - in.before;
-  ChunkPlace out;
-  out.s = place.sequence;
-  out.t = in.sequence;
-  out.kv_head = static_cast<int>(rest / blocks);
-  out.block = static_cast<int>(rest - static_cast<int64_t>(out.kv_head) * blocks);
-  out.tile_begin = unit - out.block;
-  return out;
 }
 
 // One segment: the part of a (tile, KV head) that one CTA does.
@@ -162,19 +137,27 @@ __device__ __forceinline__ bool walk_next(Walk& w, const ChunkArgs& c) {
     w.kv_head = 0;
     if (++w.t * 2 * c.half_tokens >= w.seq.q_len) {
       w.t = 0;
-      do {  // units remain, so a sequence with new tokens follows
+      do {  // units remain, so a sequence of this form follows
         w.seq = paged_sequence(c.a.batch, ++w.s, nullptr);
-      } while (w.seq.q_len == 0 && w.s + 1 < c.a.batch.sequences);
+      } while (w.seq.q_len <= c.few && w.s + 1 < c.a.batch.sequences);
     }
   }
   walk_tile(w, c);
   return true;
 }
 
+// Of a pair of 16-bit values, the sign bits of those that are not finite (exponent all ones: adding
+// one to it carries into the sign's place).
 template <typename T>
-__device__ __forceinline__ bool nonfinite_half(uint32_t bits) {
-  constexpr uint32_t kExponent = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
-  return (bits & kExponent) == kExponent;
+__device__ __forceinline__ uint32_t nonfinite_pair(uint32_t pair) {
+  constexpr uint32_t kExponents = std::is_same_v<T, __half> ? 0x7C007C00u : 0x7F807F80u;
+  constexpr uint32_t kOnes = std::is_same_v<T, __half> ? 0x04000400u : 0x00800080u;
+  return ((pair & kExponents) + kOnes) & 0x80008000u;
+}
+// The pair with its values that are not finite cleared.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_pair(uint32_t pair) {
+  return pair & ~((nonfinite_pair<T>(pair) >> 15) * 0xffffu);
 }
 
 // Sum of the values of column `column` that are not finite, over the keys [first, last] of sequence s.
@@ -232,23 +215,38 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_map(&k_map);
     prefetch_map(&v_map);
   }
-  // the part of this CTA (the barriers inside also cover the set-up above)
-  const int64_t total =
-      plan_total<kThreads>(a.batch.sequences, ctl.plan, [&](int s) { return chunk_units(c, s); });
-  const int parts = plan_parts(total, gridDim.x);
+  wait_for_producer();
   release_dependents();  // the joining kernel waits for this one's completion by itself
-  if (blockIdx.x >= parts) return;
-  const int64_t begin = part_begin(total, blockIdx.x, parts);
+  // the part of this CTA (the barriers inside also cover the set-up above)
+  const PartialSums<2 * kRows, kDim> partials(a.workspace, gridDim.x);
   Walk w;
   {
-    const ChunkPlace place = chunk_locate<kThreads>(c, begin, ctl.plan);
-    w.s = place.s;
-    w.t = place.t;
-    w.kv_head = place.kv_head;
-    w.block = place.block;
-    w.left = part_begin(total, blockIdx.x + 1, parts) - begin;
-    w.seq = paged_sequence(a.batch, w.s, nullptr);
+    PlanPlace place;
+    const bool has_part = plan_part<kThreads>(
+        a.batch, a.status, gridDim.x, ctl.plan, [&](const PagedSequence& seq) { return chunk_units(c, seq); }, place);
+    if (!has_part) {
+      if (tid == 0) leave_join_tile(partials.tiles, nullptr, 0, 0, 0, 0);
+      return;
+    }
+    const int step = 2 * c.half_tokens;
+    const int64_t begin = place.cut.begin(blockIdx.x);
+    int64_t before;
+    w.t = plan_find<kThreads>(
+        (place.seq.q_len + step - 1) / step, begin - place.before, ctl.plan,
+        [&](int t) {
+          return static_cast<int64_t>(chunk_tile(place.seq.q_len, place.seq.kv_len, step, window, t).blocks) *
+                 a.cache.kv_heads;
+        },
+        before);
+    w.s = place.sequence;
+    w.seq = place.seq;
+    w.left = place.cut.begin(blockIdx.x + 1) - begin;
+    const int blocks = chunk_tile(w.seq.q_len, w.seq.kv_len, step, window, w.t).blocks;
+    const int64_t rest = begin - place.before - before;
+    w.kv_head = static_cast<int>(PlanCut::divide(rest, blocks));
+    w.block = static_cast<int>(rest - static_cast<int64_t>(w.kv_head) * blocks);
     walk_tile(w, c);
+    if (tid == 0) leave_join_tile(partials.tiles, &place, w.t, w.kv_head, begin - w.block, blocks);
   }
   if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_base)),
@@ -450,7 +448,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t o_tmem = tmem + kTmemO + half * 128 + lane_base;
     const int row_token = row / group;
     const int row_head = row - row_token * group;
-    const PartialSums<2 * kRows, kDim> partials(a.workspace, gridDim.x);
     uint32_t turn = 0;
     uint32_t outputs = 0;  // phases of o_full so far: one a block, one a segment without any
     uint32_t segment = 0;
@@ -488,20 +485,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 4
           for (int i = tid; i < static_cast<int>(kOperand / 16); i += 2 * kRows) {
             const int key = key0 + ((i >> 3) & (kChunkBlock - 1));  // eight chunks of 16 bytes a row
-            const bool in = key >= w.tile.first_key && key <= w.tile.last_position;
-            uint4 value = v[i];
-            uint32_t* words = reinterpret_cast<uint32_t*>(&value);
-            bool change = !in;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const bool low = nonfinite_half<T>(words[j]);
-              const bool high = nonfinite_half<T>(words[j] >> 16);
-              bad |= in && (low || high);
-              change |= low || high;
-              words[j] = in ? (low ? 0u : words[j] & 0xffffu) | (high ? 0u : words[j] & 0xffff0000u) : 0u;
+            if (key < w.tile.first_key || key > w.tile.last_position) {
+              v[i] = make_uint4(0u, 0u, 0u, 0u);
+              continue;
             }
-            if (change) v[i] = value;
+            uint4 value = v[i];
+            if (nonfinite_pair<T>(value.x) | nonfinite_pair<T>(value.y) | nonfinite_pair<T>(value.z) |
+                nonfinite_pair<T>(value.w)) {
+              bad = true;
+              value.x = finite_pair<T>(value.x);
+              value.y = finite_pair<T>(value.y);
+              value.z = finite_pair<T>(value.z);
+              value.w = finite_pair<T>(value.w);
+              v[i] = value;
+            }
           }
+          __syncwarp();
           if (bad) atomicOr(&ctl.poison, 1u << (segment & 31));
           fence_async_shared();
           __syncwarp();
@@ -530,9 +529,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!whole) {
           const int low = row_first - key0;
           const int high = row_last - key0;
+          if (__any_sync(0xffffffffu, high < kChunkBlock - 1)) {
 #pragma unroll
-          for (int i = 0; i < kChunkBlock; ++i) {
-            if (i < low || i > high) x[i] = -INFINITY;
+            for (int i = 0; i < kChunkBlock; ++i) x[i] = i > high ? -INFINITY : x[i];
+          }
+          if (__any_sync(0xffffffffu, low > 0)) {
+#pragma unroll
+            for (int i = 0; i < kChunkBlock; ++i) x[i] = i < low ? -INFINITY : x[i];
           }
         }
         float top[kChains];
@@ -730,39 +733,28 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the parts of the tile that the boundary between CTAs c and c + 1 cuts, for the first such
-// boundary of each tile, in the order of the CTAs; blockIdx.y: kJoinRows of the tile's rows.
+// Joins the parts of the tile that the beginning of part blockIdx.x + 1 cuts, in the order of the CTAs;
+// blockIdx.y: kJoinRows of the tile's rows.
 template <typename T, int kDim>
 __global__ void __launch_bounds__(kJoinThreads) paged_attention_chunk_join_kernel(const ChunkArgs c, int ctas) {
-  __shared__ PlanScratch<kJoinThreads> plan;
-  const PagedAttentionArgs& a = c.a;
-  const int64_t total = plan_total<kJoinThreads>(a.batch.sequences, plan, [&](int s) { return chunk_units(c, s); });
-  const int parts = plan_parts(total, ctas);
-  const int boundary = blockIdx.x;
-  bool cut = boundary + 1 < parts;
-  ChunkPlace place{};
-  PagedSequence seq{};
-  int last = 0;  // part that holds the tile's last unit
-  if (cut) {
-    const int64_t at = part_begin(total, boundary + 1, parts);
-    place = chunk_locate<kJoinThreads>(c, at, plan);
-    seq = paged_sequence(a.batch, place.s, nullptr);
-    const int blocks = chunk_tile(seq.q_len, seq.kv_len, 2 * c.half_tokens, a.sliding_window, place.t).blocks;
-    cut = place.block > 0 && part_begin(total, boundary, parts) <= place.tile_begin;
-    last = part_of(total, place.tile_begin + blocks - 1, parts);
-  }
-  // every CTA waits, so that this grid does not complete before the one whose sums it reads
+  // every thread waits, so that this grid does not complete before the one whose sums it reads
   wait_for_producer();
-  if (!cut) return;
-  const int group = a.query_heads / a.cache.kv_heads;
+  release_dependents();
+  const PagedAttentionArgs& a = c.a;
   const PartialSums<2 * kRows, kDim> partials(a.workspace, ctas);
+  const JoinTile place = partials.tiles[blockIdx.x + 1];
+  const int last = place.last;
+  if (last < 0) return;
+  const PagedSequence seq = place.seq;
+  const int boundary = blockIdx.x;  // the part in which the tile begins
+  const int group = a.query_heads / a.cache.kv_heads;
   constexpr int kBatch = 4;  // parts whose loads are in flight together
   // a warp takes 32 rows of eight columns
   const int tile_row = blockIdx.y * kJoinRows + (threadIdx.x & 31);
   const int half = tile_row / kRows;
   const int row = tile_row - half * kRows;
   const int row_token = row / group;
-  const int token = (place.t * 2 + half) * c.half_tokens + row_token;
+  const int token = (place.tile * 2 + half) * c.half_tokens + row_token;
   if (row_token >= c.half_tokens || token >= seq.q_len) return;
   const int head = place.kv_head * group + row - row_token * group;
   for (int column = (threadIdx.x >> 5) * 8; column < kDim; column += kJoinThreads / 32 * 8) {
@@ -829,7 +821,7 @@ bool encode_map(CUtensorMap* map, int rank, const void* base, const cuuint64_t* 
 }
 
 template <typename T, int kDim>
-cudaError_t launch_chunk(const PagedAttentionArgs& a, cudaStream_t stream) {
+cudaError_t launch_chunk(const PagedAttentionArgs& a, int few, cudaStream_t stream) {
   static_assert(Layout<kDim>::bytes() <= 227 * 1024, "one CTA's shared memory");
   int device = 0;
   cudaGetDevice(&device);
@@ -845,6 +837,7 @@ cudaError_t launch_chunk(const PagedAttentionArgs& a, cudaStream_t stream) {
   ChunkArgs c;
   c.a = a;
   c.half_tokens = kRows / group;
+  c.few = few;
   const uint32_t format = std::is_same_v<T, __half> ? 0u : 1u;
   c.idesc_s = idesc(format, false, kChunkBlock);
   c.idesc_o = idesc(format, true, kDim);
@@ -863,32 +856,23 @@ cudaError_t launch_chunk(const PagedAttentionArgs& a, cudaStream_t stream) {
     return cudaErrorInvalidValue;
   }
   const int ctas = sm_count();
-  paged_attention_chunk_kernel<T, kDim><<<ctas, kThreads, Layout<kDim>::bytes(), stream>>>(q_map, k_map, v_map, c);
-  cudaError_t status = cudaGetLastError();
+  const cudaError_t status = launch_overlapped(paged_attention_chunk_kernel<T, kDim>, dim3(ctas), dim3(kThreads),
+                                               Layout<kDim>::bytes(), stream, q_map, k_map, v_map, c);
   if (status != cudaSuccess || ctas < 2) return status;
-  cudaLaunchAttribute attribute;
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(ctas - 1, 2 * kRows / kJoinRows);
-  config.blockDim = dim3(kJoinThreads);
-  config.stream = stream;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
-  status = cudaLaunchKernelEx(&config, paged_attention_chunk_join_kernel<T, kDim>, c, ctas);
-  return status != cudaSuccess ? status : cudaGetLastError();
+  return launch_overlapped(paged_attention_chunk_join_kernel<T, kDim>, dim3(ctas - 1, 2 * kRows / kJoinRows),
+                           dim3(kJoinThreads), 0, stream, c, ctas);
 }
 
 }  // namespace
 
 int64_t paged_attention_chunk_workspace(int head_dim) { return partial_bytes(2 * kRows, head_dim, sm_count()); }
 
-cudaError_t launch_paged_attention_chunk(const PagedAttentionArgs& a, cudaStream_t stream) {
+cudaError_t launch_paged_attention_chunk(const PagedAttentionArgs& a, int few, cudaStream_t stream) {
   if (a.cache.dtype == kActFp16) {
-    return a.cache.head_dim == 128 ? launch_chunk<__half, 128>(a, stream) : launch_chunk<__half, 64>(a, stream);
+    return a.cache.head_dim == 128 ? launch_chunk<__half, 128>(a, few, stream) : launch_chunk<__half, 64>(a, few, stream);
   }
-  return a.cache.head_dim == 128 ? launch_chunk<__nv_bfloat16, 128>(a, stream)
-                                 : launch_chunk<__nv_bfloat16, 64>(a, stream);
+  return a.cache.head_dim == 128 ? launch_chunk<__nv_bfloat16, 128>(a, few, stream)
+                                 : launch_chunk<__nv_bfloat16, 64>(a, few, stream);
 }
 
 }  // namespace arb

@@ -5,22 +5,22 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
+
+#include "paged.h"
 
 namespace arb {
 
-struct PlanPlace {
-  int sequence;
-  int64_t before;  // units before the sequence
-};
+#ifdef __CUDACC__
 
 template <int kCount>  // threads of the block, a multiple of 32
 struct PlanScratch {
   int64_t sums[kCount / 32];
-  PlanPlace place;
+  int64_t before;  // units before the sequence (or tile) that was found
+  PagedSequence seq;
+  int index;
 };
-
-#ifdef __CUDACC__
 
 // Inclusive sum over the block's threads, and the block's total.
 template <int kCount>
@@ -41,67 +41,156 @@ __device__ __forceinline__ int64_t plan_scan(int64_t mine, int64_t& total, PlanS
     if (w == warp) sum += total;
     total += scratch.sums[w];
   }
-  __syncthreads();
   return sum;
 }
 
-// Units of the whole batch; units(s) gives a sequence's.
-template <int kCount, typename Units>
-__device__ __forceinline__ int64_t plan_total(int sequences, PlanScratch<kCount>& scratch, Units units) {
-  int64_t mine = 0;
-  for (int s = threadIdx.x; s < sequences; s += kCount) mine += units(s);
+// The line's cut into parts, one a CTA, each of at least one unit: the first `longer` parts have one
+// unit more than the others.
+struct PlanCut {
   int64_t total;
-  plan_scan<kCount>(mine, total, scratch);
-  return total;
+  int parts;
+  int longer;
+  int64_t length;
+  __device__ __forceinline__ int64_t begin(int part) const { return length * part + min(part, longer); }
+  __device__ __forceinline__ int part_of(int64_t unit) const {
+    const int64_t in_longer = (length + 1) * longer;
+    return unit < in_longer ? static_cast<int>(divide(unit, length + 1))
+                            : longer + static_cast<int>(divide(unit - in_longer, length));
+  }
+  // 32-bit where that does: a 64-bit division takes four times as long
+  static __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+    if ((a | b) >> 32 == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+  }
+};
+
+// What a CTA's part begins with.
+struct PlanPlace {
+  PlanCut cut;
+  int sequence;
+  int64_t before;  // units before the sequence
+  PagedSequence seq;
+};
+
+// Cuts the batch for `ctas` CTAs and finds where part blockIdx.x begins; units(seq) gives a sequence's.
+// False: this CTA has no part. The whole block calls it.
+template <int kCount, typename Units>
+__device__ __forceinline__ bool plan_part(const PagedBatch& b, int* status, int ctas, PlanScratch<kCount>& scratch,
+                                          Units units, PlanPlace& place) {
+  const int s = threadIdx.x;
+  PagedSequence seq = s < b.sequences ? paged_sequence(b, s, status) : PagedSequence{0, 0, 0};
+  int64_t mine = units(seq);
+  int64_t all;
+  int64_t sum = plan_scan<kCount>(mine, all, scratch);
+  PlanCut& cut = place.cut;
+  cut.total = all;
+  for (int base = kCount; base < b.sequences; base += kCount) {  // more sequences than threads
+    int64_t more;
+    __syncthreads();
+    plan_scan<kCount>(base + s < b.sequences ? units(paged_sequence(b, base + s, status)) : 0, more, scratch);
+    cut.total += more;
+  }
+  cut.parts = static_cast<int>(min(cut.total, static_cast<int64_t>(ctas)));
+  if (static_cast<int>(blockIdx.x) >= cut.parts) return false;
+  cut.length = PlanCut::divide(cut.total, cut.parts);
+  cut.longer = static_cast<int>(cut.total - cut.length * cut.parts);
+  const int64_t unit = cut.begin(blockIdx.x);
+  int64_t before = 0;
+  for (int base = 0;; base += kCount) {
+    if (unit >= before + sum - mine && unit < before + sum) {
+      scratch.index = base + s;
+      scratch.before = before + sum - mine;
+      scratch.seq = seq;
+    }
+    before += all;
+    if (unit < before || base + kCount >= b.sequences) break;
+    const int next = base + kCount + s;
+    seq = next < b.sequences ? paged_sequence(b, next, nullptr) : PagedSequence{0, 0, 0};
+    mine = units(seq);
+    __syncthreads();
+    sum = plan_scan<kCount>(mine, all, scratch);
+  }
+  __syncthreads();
+  place.sequence = scratch.index;
+  place.before = scratch.before;
+  place.seq = scratch.seq;
+  return true;
 }
 
-// The sequence that holds unit `unit` (below the total).
+// The index i < count whose units hold `unit`, and the units before it; the whole block calls it.
 template <int kCount, typename Units>
-__device__ __forceinline__ PlanPlace plan_locate(int sequences, int64_t unit, PlanScratch<kCount>& scratch, Units units) {
+__device__ __forceinline__ int plan_find(int count, int64_t unit, PlanScratch<kCount>& scratch, Units units,
+                                         int64_t& before_it) {
   int64_t before = 0;
-  for (int base = 0; base < sequences; base += kCount) {
-    const int s = base + threadIdx.x;
-    const int64_t mine = s < sequences ? units(s) : 0;
+  for (int base = 0; base < count; base += kCount) {
+    const int i = base + threadIdx.x;
+    const int64_t mine = i < count ? units(i) : 0;
     int64_t all;
+    __syncthreads();
     const int64_t sum = before + plan_scan<kCount>(mine, all, scratch);
-    if (unit >= sum - mine && unit < sum) scratch.place = {s, sum - mine};
+    if (unit >= sum - mine && unit < sum) {
+      scratch.index = i;
+      scratch.before = sum - mine;
+    }
     before += all;
     if (unit < before) break;
   }
   __syncthreads();
-  return scratch.place;
+  before_it = scratch.before;
+  return scratch.index;
 }
 
-// Parts the line is cut into: one a CTA, each of at least one unit.
-__device__ __forceinline__ int plan_parts(int64_t total, int ctas) {
-  return static_cast<int>(min(total, static_cast<int64_t>(ctas)));
-}
-// Where part c of `parts` begins, and the part that holds a unit.
-__device__ __forceinline__ int64_t part_begin(int64_t total, int c, int parts) { return total * c / parts; }
-__device__ __forceinline__ int part_of(int64_t total, int64_t unit, int parts) {
-  return static_cast<int>(((unit + 1) * parts - 1) / total);
-}
+// What the joining kernel needs about the tile that the beginning of a CTA's part cuts; written by
+// every CTA, `last` is below 0 where there is nothing to join (the part begins with a tile, does not
+// exist, or another CTA's beginning cuts the tile first).
+struct JoinTile {
+  int last;  // the part that holds the tile's last unit
+  int sequence;
+  int tile;
+  int kv_head;
+  PagedSequence seq;
+  int unused;
+};
 
-// Partial sums of a tile that several CTAs share. A CTA has two slots: 1 for a tile that begins in its
-// part, 0 for one that began before it.
+// Partial sums of a tile that several CTAs share, and what to join. A CTA has two slots: 1 for a tile
+// that begins in its part, 0 for one that began before it.
 template <int kRows, int kDim>
 struct PartialSums {
-  float* sums;    // [2 ctas][kRows][kDim], not divided by the rows' sums
-  float2* stats;  // [2 ctas][kRows]: reference and sum
+  float* sums;      // [2 ctas][kRows * kDim], not divided by the rows' sums
+  float2* stats;    // [2 ctas][kRows]: reference and sum
+  JoinTile* tiles;  // [ctas]
   __device__ __forceinline__ PartialSums(void* workspace, int ctas)
       : sums(static_cast<float*>(workspace)),
-        stats(reinterpret_cast<float2*>(sums + static_cast<int64_t>(2) * ctas * kRows * kDim)) {}
+        stats(reinterpret_cast<float2*>(sums + static_cast<int64_t>(2) * ctas * kRows * kDim)),
+        tiles(reinterpret_cast<JoinTile*>(stats + static_cast<int64_t>(2) * ctas * kRows)) {}
 };
+
+// One thread of each CTA leaves its JoinTile. `tile_begin` is the unit at which the tile of the part's
+// first unit begins.
+__device__ __forceinline__ void leave_join_tile(JoinTile* tiles, const PlanPlace* place, int tile, int kv_head,
+                                                int64_t tile_begin, int blocks) {
+  JoinTile join{};
+  join.last = -1;
+  const int part = blockIdx.x;
+  if (place != nullptr && part > 0 && tile_begin < place->cut.begin(part) && tile_begin >= place->cut.begin(part - 1)) {
+    join.last = place->cut.part_of(tile_begin + blocks - 1);
+    join.sequence = place->sequence;
+    join.tile = tile;
+    join.kv_head = kv_head;
+    join.seq = place->seq;
+  }
+  tiles[part] = join;
+}
 
 #endif  // __CUDACC__
 
 constexpr int64_t partial_bytes(int rows, int dim, int ctas) {
-  return static_cast<int64_t>(2) * ctas * rows * (dim * sizeof(float) + sizeof(float2));
+  return static_cast<int64_t>(ctas) * (2 * rows * (dim * sizeof(float) + sizeof(float2)) + 32);
 }
 
 // sum over i < n of floor((a i + b) / m), by Euclid's algorithm on (m, a): whole multiples of m leave
 // closed sums, and counting the lattice points below the line that remains by columns instead of rows
-// swaps m and a.
+// swaps m and a. Everything stays below 2^32: n < 2^25 and, after the first step, a, b < m <= 256.
 __host__ __device__ inline int64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
   int64_t sum = 0;
   while (n > 0) {
@@ -109,10 +198,10 @@ __host__ __device__ inline int64_t floor_sum(uint32_t n, uint32_t m, uint32_t a,
     sum += static_cast<int64_t>(n) * (n - 1) / 2 * a_whole + static_cast<int64_t>(n) * b_whole;
     a -= a_whole * m;
     b -= b_whole * m;
-    const uint64_t top = static_cast<uint64_t>(a) * n + b;
+    const uint32_t top = a * n + b;
     if (top < m) break;
-    n = static_cast<uint32_t>(top / m);
-    b = static_cast<uint32_t>(top - static_cast<uint64_t>(n) * m);
+    n = top / m;
+    b = top - n * m;
     const uint32_t swap = m;
     m = a;
     a = swap;
