@@ -152,7 +152,7 @@ __device__ float nonfinite_sum(const PagedAttentionArgs& a, int s, int kv_head, 
 template <typename T, int kGroups, int kDim>
 __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<kGroups, kDim>::kCtasPerSm)
     paged_attention_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                               const PagedAttentionArgs a, int most) {
+                               const __grid_constant__ PagedAttentionArgs a, int most) {
   using Shared = FewShared<kGroups, kDim>;
   constexpr int kThreads = Shared::kThreads;
   constexpr int kStages = Shared::kStages;

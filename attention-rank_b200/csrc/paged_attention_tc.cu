@@ -4,10 +4,10 @@
 // Rows: the query heads of a KV head are stacked, row = token * group + head, so that they share each
 // K and V tile and the causal edge of a tile stays a few tokens wide. A tile is two M = 128 halves of
 // floor(128 / group) tokens each; K and V come in 128-key blocks, one or more pages each, by TMA.
-// One persistent CTA an SM, 384 threads:
+// One persistent CTA an SM, 320 threads:
 //   warps 0-3, 4-7  softmax of half 0 / 1: thread r owns row r (TMEM lane r) of its half
 //   warp 8          TMA: Q of both halves, K and V blocks into a ring of four stages
-//   warp 9          tcgen05.mma of both halves (warps 10 and 11 only fill up the warpgroup)
+//   warp 9          tcgen05.mma of both halves
 // TMEM: S0 | S1 | O0 | O1, 128 columns each; P (16-bit) overwrites its S. Per half and block:
 //   S = Q K^T;  softmax warps read S, write P in two halves of 64 keys;  O += P V starts with the first
 //   while the second is being computed;  the next S follows behind it.
@@ -40,10 +40,7 @@ using namespace async;
 using namespace tc;
 
 constexpr int kRows = 128;                          // rows of a half tile
-constexpr int kThreads = 384;
-// setmaxnreg shares of the 384 x 168 registers of the launch: 256 x 208 + 128 x 80 = 63488 <= 64512
-constexpr int kSoftmaxRegisters = 208;
-constexpr int kIssueRegisters = 80;
+constexpr int kThreads = 320;
 constexpr int kStages = 4;
 constexpr uint32_t kHalfBytes = 128 * 128;          // 128 rows of 64 16-bit values
 constexpr uint32_t kTmemColumns = 512;
@@ -51,7 +48,6 @@ constexpr uint32_t kTmemO = 256;
 constexpr int kJoinThreads = 256;
 constexpr int kJoinRows = 32;                       // rows of a tile that one joining CTA takes
 constexpr float kRescaleThreshold = 8.0f;           // log2 units
-constexpr int kFmaPairs = 0;                        // of 8 pairs of exponentials, those on the FMA pipe
 constexpr int kChains = 4;                          // independent accumulators per row reduction
 
 struct __align__(16) Control {
@@ -160,25 +156,33 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t pair) {
   return pair & ~((nonfinite_pair<T>(pair) >> 15) * 0xffffu);
 }
 
-// Sum of the values of column `column` that are not finite, over the keys [first, last] of sequence s.
+// Adds to a row, written by this thread, the values of V that are not finite at the keys [first, last]
+// it sees. `out` is the row in the 16-bit result, or NULL and `sums` its place in the partial sums.
 template <typename T, int kDim>
-__device__ __noinline__ float nonfinite_sum(const PagedAttentionArgs& a, int s, int kv_head, int first, int last,
-                                            int column) {
-  float sum = 0.0f;
-  for (int key = first; key <= last; ++key) {
-    const int page = paged_page(a.cache, a.batch, s, key >> a.cache.page_shift, a.status);
-    const int64_t row = ((static_cast<int64_t>(page) * a.cache.kv_heads + kv_head) << a.cache.page_shift) +
-                        (key & ((1 << a.cache.page_shift) - 1));
-    const float v = static_cast<float>(static_cast<const T*>(a.cache.v_pages)[row * kDim + column]);
-    if (!isfinite(v)) sum += v;
+__device__ __noinline__ void add_nonfinite(const PagedAttentionArgs& a, int s, int kv_head, int first, int last, T* out,
+                                           float* sums) {
+  for (int column = 0; column < kDim; ++column) {
+    float more = 0.0f;
+    for (int key = first; key <= last; ++key) {
+      const int page = paged_page(a.cache, a.batch, s, key >> a.cache.page_shift, a.status);
+      const int64_t row = ((static_cast<int64_t>(page) * a.cache.kv_heads + kv_head) << a.cache.page_shift) +
+                          (key & ((1 << a.cache.page_shift) - 1));
+      const float v = static_cast<float>(static_cast<const T*>(a.cache.v_pages)[row * kDim + column]);
+      if (!isfinite(v)) more += v;
+    }
+    if (more == 0.0f) continue;  // all of them finite
+    if (out != nullptr) {
+      out[column] = static_cast<T>(static_cast<float>(out[column]) + more);
+    } else {
+      sums[(column >> 2) * (2 * kRows * 4) + (column & 3)] += more;
+    }
   }
-  return sum;
 }
 
 template <typename T, int kDim>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-                                 const __grid_constant__ CUtensorMap v_map, const ChunkArgs c) {
+                                 const __grid_constant__ CUtensorMap v_map, const __grid_constant__ ChunkArgs c) {
   constexpr uint32_t kOperand = Layout<kDim>::kOperand;
   constexpr int kHalves = kDim / 64;
   extern __shared__ uint8_t smem_raw[];
@@ -264,8 +268,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto phase_of = [](uint32_t item) { return (item / kStages) & 1; };
   bool ok = true;
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegisters));
   if (warp == 8) {
     // ------------------------------------------------------------------------------------- TMA
     const int page_rows = min(1 << a.cache.page_shift, kChunkBlock);
@@ -339,36 +341,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The halves' products are issued in turn, [O += P V, next S] of half 0, then of half 1, which keeps
     // the halves half a block apart: with a warp for each half they fell into step, their exponentials
     // sharing the SFU and their products the tensor pipe (985 against 735 us for two 4K chunks).
+    const uint32_t elected = elect_one();
     uint32_t turn = 0;  // blocks so far
     uint32_t segment = 0;
-    uint32_t cleaned[2] = {0, 0};
+    uint32_t cleaned = 0;  // the next phases of the two `clean` barriers, a bit each
     do {
-      int h_begin[2], h_end[2];
-      w.half_range(0, half_tokens, window, h_begin[0], h_end[0]);
-      w.half_range(1, half_tokens, window, h_begin[1], h_end[1]);
+      int begin0, end0, begin1, end1;
+      w.half_range(0, half_tokens, window, begin0, end0);
+      w.half_range(1, half_tokens, window, begin1, end1);
       const int end = w.block + w.count;
+      auto needs = [&](int half, int b) { return half == 0 ? b >= begin0 && b < end0 : b >= begin1 && b < end1; };
       // S = Q K^T of block b (the n-th of the part) where the half needs it
       auto scores = [&](int half, int b, uint32_t n) {
-        if (elect_one()) {
-          if (b >= h_begin[half] && b < h_end[half]) {
-            const uint32_t q_at = q_smem + half * kOperand;
-            const uint32_t k_at = ring + stage_of(2 * n) * kOperand;
+        if (needs(half, b)) {
+          const uint64_t q_at = desc_k_major(q_smem + half * kOperand);
+          const uint64_t k_at = desc_k_major(ring + stage_of(2 * n) * kOperand);
 #pragma unroll
-            for (int k = 0; k < kDim / 16; ++k) {
-              const uint32_t offset = (k >> 2) * kHalfBytes + (k & 3) * 32;
-              mma_ss(tmem + half * 128, desc_k_major(q_at + offset), desc_k_major(k_at + offset), c.idesc_s,
-                     k > 0 ? 1u : 0u);
-            }
-            mma_commit(smem_u32(&ctl.s_full[half]));
-          } else {
-            mbar_arrive(smem_u32(&ctl.s_full[half]));
+          for (int k = 0; k < kDim / 16; ++k) {  // 16 values, 32 bytes of a row, a step
+            const uint64_t offset = (k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2;
+            mma_ss(elected, tmem + half * 128, q_at + offset, k_at + offset, c.idesc_s, k > 0 ? 1u : 0u);
           }
-          if (half == 1) {
-            mma_commit(smem_u32(&ctl.empty[stage_of(2 * n)]));
-            if (b == end - 1) mma_commit(smem_u32(&ctl.q_empty));  // Q has been read for the last time
-          }
+          mma_commit(elected, smem_u32(&ctl.s_full[half]));
+        } else {
+          mbar_arrive_if(elected, smem_u32(&ctl.s_full[half]));
         }
-        __syncwarp();
+        if (half == 1) {
+          mma_commit(elected, smem_u32(&ctl.empty[stage_of(2 * n)]));
+          if (b == end - 1) mma_commit(elected, smem_u32(&ctl.q_empty));  // Q has been read for the last time
+        }
       };
       auto wait_k = [&](uint32_t n) {
         const bool there = mbar_wait(smem_u32(&ctl.full[stage_of(2 * n)]), phase_of(2 * n), &ctl.abort);
@@ -379,41 +379,38 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       scores(0, w.block, turn);
       scores(1, w.block, turn);
-      bool waited_o[2] = {segment == 0, segment == 0};
+      uint32_t waited_o = segment == 0 ? 3u : 0u;  // halves whose O of the last segment has been read
       for (int b = w.block; ok && b < end; ++b, ++turn) {
         const uint32_t v_item = 2 * turn + 1;
         const uint32_t stage = stage_of(v_item);
         ok = mbar_wait(smem_u32(&ctl.full[stage]), phase_of(v_item), &ctl.abort);
         if (ok && !w.whole(b, window)) {  // V of this block is cleared by the softmax warps first
-          ok = mbar_wait(smem_u32(&ctl.clean[turn & 1]), cleaned[turn & 1] & 1, &ctl.abort);
-          ++cleaned[turn & 1];
+          ok = mbar_wait(smem_u32(&ctl.clean[turn & 1]), (cleaned >> (turn & 1)) & 1, &ctl.abort);
+          cleaned ^= 1u << (turn & 1);
         }
-        const uint32_t v_at = ring + stage * kOperand;
+        const uint64_t v_at = desc_mn_major(ring + stage * kOperand, kHalfBytes);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const bool needed = b >= h_begin[half] && b < h_end[half];
-          if (ok && needed && !waited_o[half]) {  // the last segment's O has been read
+          const bool needed = needs(half, b);
+          if (ok && needed && !(waited_o >> half & 1)) {
             ok = mbar_wait(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
-            waited_o[half] = true;
+            waited_o |= 1u << half;
           }
 #pragma unroll
           for (int part = 0; part < 2; ++part) {
             ok = ok && mbar_wait(smem_u32(&ctl.p_full[half][part]), turn & 1, &ctl.abort);
             fence_after();
-            if (ok && elect_one()) {
-              if (needed) {
+            if (ok && needed) {
+              const bool first = b == (half == 0 ? begin0 : begin1);
 #pragma unroll
-                for (int k = part * 4; k < part * 4 + 4; ++k) {
-                  mma_ts(tmem + kTmemO + half * 128, tmem + half * 128 + k * 8,
-                         desc_mn_major(v_at + k * 16 * 128, kHalfBytes), c.idesc_o,
-                         (b > h_begin[half] || k > 0) ? 1u : 0u);
-                }
-                if (part == 1) mma_commit(smem_u32(&ctl.o_full[half]));
+              for (int k = part * 4; k < part * 4 + 4; ++k) {  // 16 keys a step
+                mma_ts(elected, tmem + kTmemO + half * 128, tmem + half * 128 + k * 8, v_at + k * (16 * 128 >> 4),
+                       c.idesc_o, first && k == 0 ? 0u : 1u);
               }
-              if (half == 1 && part == 1) mma_commit(smem_u32(&ctl.empty[stage]));
+              if (part == 1) mma_commit(elected, smem_u32(&ctl.o_full[half]));
             }
-            __syncwarp();
           }
+          if (ok && half == 1) mma_commit(elected, smem_u32(&ctl.empty[stage]));
           if (ok && b + 1 < end) {
             if (half == 0) ok = wait_k(turn + 1);
             if (ok) scores(half, b + 1, turn + 1);
@@ -422,10 +419,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        if (ok && !waited_o[half]) ok = mbar_wait(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
+        if (ok && !(waited_o >> half & 1)) ok = mbar_wait(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
         // a half without blocks takes part too, so that its softmax warps stay within a segment of it
-        if (ok && h_begin[half] == h_end[half] && lane == 0) mbar_arrive(smem_u32(&ctl.o_full[half]));
-        __syncwarp();
+        if (ok && (half == 0 ? begin0 == end0 : begin1 == end1)) mbar_arrive_if(elected, smem_u32(&ctl.o_full[half]));
       }
       ++segment;
     } while (ok && walk_next(w, c));
@@ -434,13 +430,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       ctl.abort = 1;
     }
     // every MMA has completed before TMEM and shared memory are released
-    __syncwarp();
-    if (elect_one()) mma_commit(smem_u32(&ctl.done));
+    mma_commit(elected, smem_u32(&ctl.done));
     mbar_wait(smem_u32(&ctl.done), 0, nullptr);
-  }
   } else {
     // --------------------------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
     const int half = warp >> 2;
     const int row = tid & (kRows - 1);
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -449,9 +442,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int row_token = row / group;
     const int row_head = row - row_token * group;
     uint32_t turn = 0;
+    const uint32_t elected = lane == 0 ? 1u : 0u;
     uint32_t outputs = 0;  // phases of o_full so far: one a block, one a segment without any
     uint32_t segment = 0;
-    uint32_t cleaned[2] = {0, 0};
+    uint32_t cleaned = 0;       // the next phases of the two `clean` barriers, a bit each
+    uint32_t cleaned_once = 0;  // which of them have had one
     do {
       int h_begin, h_end;
       w.half_range(half, half_tokens, window, h_begin, h_end);
@@ -504,48 +499,44 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (bad) atomicOr(&ctl.poison, 1u << (segment & 31));
           fence_async_shared();
           __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&ctl.clean[turn & 1]));
-          __syncwarp();
-          ++cleaned[turn & 1];
+          mbar_arrive_if(elected, smem_u32(&ctl.clean[turn & 1]));
+          cleaned ^= 1u << (turn & 1);
+          cleaned_once |= 1u << (turn & 1);
         }
         if (!needed) {
-          if (lane == 0) {
-            mbar_arrive(smem_u32(&ctl.p_full[half][0]));
-            mbar_arrive(smem_u32(&ctl.p_full[half][1]));
-          }
-          __syncwarp();
+          mbar_arrive_if(elected, smem_u32(&ctl.p_full[half][0]));
+          mbar_arrive_if(elected, smem_u32(&ctl.p_full[half][1]));
           continue;
         }
         fence_after();
-        float x[kChunkBlock];
-        {
-          uint32_t raw[4][32];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tmem_ld32(s_tmem + i * 32, raw[i]);
+        // S passes through the registers 64 columns at a time, twice: the upper and the lower half for the
+        // maximum, the lower (still there) and the upper for the probabilities. P's 16-bit pairs take the
+        // place of scores already read.
+        const int low = row_first - key0;
+        const int high = row_last - key0;
+        float x[64];
+        auto load = [&](int column) {
+          uint32_t raw[2][32];
+          tmem_ld32(s_tmem + column, raw[0]);
+          tmem_ld32(s_tmem + column + 32, raw[1]);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < kChunkBlock; ++i) x[i] = __uint_as_float(raw[i >> 5][i & 31]);
-        }
-        if (!whole) {
-          const int low = row_first - key0;
-          const int high = row_last - key0;
-          if (__any_sync(0xffffffffu, high < kChunkBlock - 1)) {
+          for (int i = 0; i < 64; ++i) x[i] = __uint_as_float(raw[i >> 5][i & 31]);
+          if (!whole) {
 #pragma unroll
-            for (int i = 0; i < kChunkBlock; ++i) x[i] = i > high ? -INFINITY : x[i];
+            for (int i = 0; i < 64; ++i) x[i] = i + column > high || i + column < low ? -INFINITY : x[i];
           }
-          if (__any_sync(0xffffffffu, low > 0)) {
-#pragma unroll
-            for (int i = 0; i < kChunkBlock; ++i) x[i] = i < low ? -INFINITY : x[i];
-          }
-        }
+        };
         float top[kChains];
 #pragma unroll
-        for (int i = 0; i < kChains; ++i) top[i] = x[i];
+        for (int i = 0; i < kChains; ++i) top[i] = -INFINITY;
+#pragma unroll 1
+        for (int column = 0; column < kChunkBlock; column += 64) {
+          load(column);
 #pragma unroll
-        for (int i = kChains; i < kChunkBlock; i += 2) {
-          top[(i / 2) % kChains] = max3_nan(top[(i / 2) % kChains], x[i], x[i + 1]);
+          for (int i = 0; i < 64; i += 2) top[(i / 2) % kChains] = max3(top[(i / 2) % kChains], x[i], x[i + 1]);
         }
-        const float block_top = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
+        const float block_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
         // the row's reference moves only when the block's maximum exceeds it by more than the threshold,
         // so probabilities stay below 2^8 and O is rarely rescaled
         const bool move = block_top > reference + kRescaleThreshold || (reference == -INFINITY && block_top != -INFINITY);
@@ -574,62 +565,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         unsigned long long sums[kChains / 2];
 #pragma unroll
         for (int i = 0; i < kChains / 2; ++i) sums[i] = 0ull;
-        // Groups of eight pairs, of which kFmaPairs run on the FMA pipe (where every score is finite): the
-        // SFU's are issued first, its results are used a group later.
-        auto probabilities = [&](auto share) {
-          constexpr int kFma = decltype(share)::value;
-          constexpr int kSfu = 8 - kFma;
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {
+          load(part * 64);
+          uint32_t packed[32];
 #pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            uint32_t packed[32];
-            float p[2][16];
-            auto finish = [&](int group) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float p0 = p[group & 1][2 * i], p1 = p[group & 1][2 * i + 1];
-                sums[i % (kChains / 2)] = add_f32x2(sums[i % (kChains / 2)], pack_f32x2(p0, p1));
-                packed[group * 8 + i] = pack2<T>(p0, p1);
-              }
-            };
-#pragma unroll
-            for (int group = 0; group < 4; ++group) {
-              unsigned long long t[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int at = part * 64 + group * 16 + 2 * i;
-                t[i] = fma_f32x2(pack_f32x2(x[at], x[at + 1]), scale2, base2);
-              }
-#pragma unroll
-              for (int i = 0; i < kSfu; ++i) {
-                float t0, t1;
-                unpack_f32x2(t[i], t0, t1);
-                p[group & 1][2 * i] = ex2_ftz(t0);
-                p[group & 1][2 * i + 1] = ex2_ftz(t1);
-              }
-              if constexpr (kFma > 0) {
-                unsigned long long rest[kFma];
-                float out[2 * kFma];
-#pragma unroll
-                for (int i = 0; i < kFma; ++i) rest[i] = t[kSfu + i];
-                exp2_fma<kFma>(rest, out);
-#pragma unroll
-                for (int i = 0; i < 2 * kFma; ++i) p[group & 1][2 * kSfu + i] = out[i];
-              }
-              if (group > 0) finish(group - 1);
-            }
-            finish(3);
-            tmem_st32(s_tmem + part * 32, packed);
-            tmem_wait_st();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&ctl.p_full[half][part]));
-            __syncwarp();
+          for (int i = 0; i < 32; ++i) {
+            float p0, p1;
+            unpack_f32x2(fma_f32x2(pack_f32x2(x[2 * i], x[2 * i + 1]), scale2, base2), p0, p1);
+            p0 = ex2_ftz(p0);
+            p1 = ex2_ftz(p1);
+            sums[i % (kChains / 2)] = add_f32x2(sums[i % (kChains / 2)], pack_f32x2(p0, p1));
+            packed[i] = pack2<T>(p0, p1);
           }
-        };
-        if (whole && __all_sync(0xffffffffu, !row_in || fabsf(block_top) < INFINITY)) {
-          probabilities(std::integral_constant<int, kFmaPairs>{});
-        } else {
-          probabilities(std::integral_constant<int, 0>{});
+          tmem_st32(s_tmem + part * 32, packed);
+          tmem_wait_st();
+          fence_before();
+          mbar_arrive_if(elected, smem_u32(&ctl.p_full[half][part]));
         }
 #pragma unroll
         for (int i = 0; i < kChains / 2; ++i) {
@@ -649,8 +601,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       // every thread's share of the cleared blocks is done when their barriers' last phases are
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (cleaned[i] > 0 && ok) {
-          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl.clean[i]), (cleaned[i] - 1) & 1, &ctl.abort));
+        if ((cleaned_once >> i & 1) && ok) {
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl.clean[i]), ((cleaned >> i) & 1) ^ 1, &ctl.abort));
         }
       }
       if (!ok) break;
@@ -671,17 +623,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) raw[j] = 0u;
-        }
-        if (row_in && poisoned) {
-          const int low = max(row_first, (w.tile.block_begin + w.block) * kChunkBlock);
-          const int high = min(row_last, (w.tile.block_begin + end) * kChunkBlock - 1);
-          for (int j = 0; j < 32; ++j) {
-            const float more = nonfinite_sum<T, kDim>(a, w.s, w.kv_head, low, high, i * 32 + j);
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              if (k == j) raw[k] = __float_as_uint(__uint_as_float(raw[k]) + more);
-            }
-          }
         }
         if (row_in && complete) {
           T* to = static_cast<T*>(a.out) + out_token * a.out_stride + head * kDim + i * 32;
@@ -707,7 +648,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&ctl.o_free[half]));
+      mbar_arrive_if(elected, smem_u32(&ctl.o_free[half]));
+      if (row_in && poisoned) {
+        add_nonfinite<T, kDim>(a, w.s, w.kv_head, max(row_first, (w.tile.block_begin + w.block) * kChunkBlock),
+                               min(row_last, (w.tile.block_begin + end) * kChunkBlock - 1),
+                               complete ? static_cast<T*>(a.out) + out_token * a.out_stride + head * kDim : nullptr,
+                               partials.sums + (slot * (2 * kRows) * (kDim / 4) + half * kRows + row) * 4);
+      }
       if (row_in) {
         if (!complete) {
           partials.stats[slot * (2 * kRows) + half * kRows + row] = make_float2(reference, l);

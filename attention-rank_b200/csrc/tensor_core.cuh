@@ -26,36 +26,42 @@ constexpr uint32_t idesc(uint32_t format, bool b_mn_major, uint32_t n) {
   return (1u << 4) | (format << 7) | (format << 10) | (b_mn_major ? (1u << 16) : 0u) | ((n >> 3) << 17) |
          ((128u >> 4) << 24);
 }
-// True in one lane of the converged warp. A warp that walks its loop as a whole and issues through
-// this keeps descriptors in uniform registers; under `if (lane == 0)` each MMA moved its operands there
-// one by one.
-__device__ __forceinline__ bool elect_one() {
+// 1 in one lane of the converged warp, 0 in the others. What follows is issued by that lane: as
+// predicated instructions, not under a branch, which would part and rejoin the warp each time.
+__device__ __forceinline__ uint32_t elect_one() {
   uint32_t elected;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "elect.sync _|p, 0xffffffff;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(elected));
-  return elected != 0;
+  return elected;
 }
 // D (TMEM) = A (shared) B (shared) (+ D)
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t elected, uint32_t d, uint64_t a, uint64_t b, uint32_t id,
+                                       uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate)
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate), "r"(elected)
       : "memory");
 }
 // D (TMEM) = A (TMEM) B (shared) (+ D)
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t id, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t elected, uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t id,
+                                       uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a_tmem), "l"(b), "r"(id), "r"(accumulate)
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a_tmem), "l"(b), "r"(id), "r"(accumulate), "r"(elected)
       : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// Arrives on the barrier once the MMAs issued so far have completed.
+__device__ __forceinline__ void mma_commit(uint32_t elected, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(bar), "r"(elected)
+      : "memory");
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -107,51 +113,11 @@ __device__ __forceinline__ unsigned long long add_f32x2(unsigned long long a, un
   asm("add.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-// max(a, b, c) in one instruction; NaN if any of them is
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+// max(a, b, c) in one instruction
+__device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
-}
-// 2^t of kPairs pairs on the FMA pipe, for finite t below 127: 2^t = 2^n 2^f, n the nearest integer
-// (found by adding 1.5 x 2^23, whose sum keeps n in its low bits), 2^f on [-1/2, 1/2] by the polynomial
-// of degree 5 with the least largest relative error (7.5e-8; 2.2e-7 with the fp32 roundings, checked at
-// 2 million points), n added to the exponent. Below 2^-125 it stays there. Step by step over all pairs,
-// so that a step's latency is hidden behind the others'.
-template <int kPairs>
-__device__ __forceinline__ void exp2_fma(const unsigned long long (&t)[kPairs], float (&p)[2 * kPairs]) {
-  unsigned long long clamped[kPairs], shifted[kPairs], f[kPairs], y[kPairs];
-  const auto both = [](float v) { return pack_f32x2(v, v); };
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i) {
-    float t0, t1;
-    unpack_f32x2(t[i], t0, t1);
-    clamped[i] = pack_f32x2(fmaxf(t0, -125.0f), fmaxf(t1, -125.0f));
-  }
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i) shifted[i] = add_f32x2(clamped[i], both(12582912.0f));
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i) f[i] = add_f32x2(shifted[i], both(-12582912.0f));
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i) f[i] = fma_f32x2(f[i], both(-1.0f), clamped[i]);
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i) y[i] = fma_f32x2(both(0.0013276472454890609f), f[i], both(0.009675541892647743f));
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i) y[i] = fma_f32x2(y[i], f[i], both(0.05550713092088699f));
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i) y[i] = fma_f32x2(y[i], f[i], both(0.24022120237350464f));
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i) y[i] = fma_f32x2(y[i], f[i], both(0.6931469440460205f));
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i) y[i] = fma_f32x2(y[i], f[i], both(1.0000001192092896f));
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i) {
-    float s0, s1, y0, y1;
-    unpack_f32x2(shifted[i], s0, s1);
-    unpack_f32x2(y[i], y0, y1);
-    p[2 * i] = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(s0) << 23));
-    p[2 * i + 1] = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(s1) << 23));
-  }
 }
 // A whole 32-byte sector in one store (two 16-byte stores each write half of one).
 __device__ __forceinline__ void store_sector(void* to, const uint32_t (&r)[8]) {
