@@ -42,20 +42,23 @@ __device__ __forceinline__ uint64_t global_ns() {
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t phase) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(phase)
+      : "memory");
+  return done != 0;
+}
 // Bounded wait for the completion of phase `phase` (parity): gives up after kWaitLimitNs (or
 // kSpinLimit polls), or earlier once *abort is set by another thread of the CTA.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t phase, const volatile int* abort) {
   uint64_t start = 0;
   for (uint32_t i = 0; i < kSpinLimit; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(phase)
-        : "memory");
-    if (done) return true;
+    if (mbar_try(bar, phase)) return true;
     if ((i & 1023) == 1023) {
       if (abort != nullptr && *abort) return false;
       const uint64_t now = global_ns();
@@ -67,6 +70,15 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t phase, const vo
     }
   }
   return false;
+}
+// The same with the loop in a function of its own, for a kernel that waits at many places with few live
+// registers: the copies of the loop crowd the instruction cache (830 -> 800 us for two 4K chunks in the
+// chunk attention; in the few-row attention, whose accumulators are live, the call spills: 193 -> 202).
+static __device__ __noinline__ bool mbar_wait_loop(uint32_t bar, uint32_t phase, const volatile int* abort) {
+  return mbar_wait(bar, phase, abort);
+}
+__device__ __forceinline__ bool mbar_wait_called(uint32_t bar, uint32_t phase, const volatile int* abort) {
+  return mbar_try(bar, phase) || mbar_wait_loop(bar, phase, abort);
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile(

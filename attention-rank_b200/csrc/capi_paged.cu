@@ -156,7 +156,7 @@ int ar_rope_table_scaled(const ar_rope_scaling* scaling, int positions, float* c
     require(scaling != nullptr, who, "null argument");
     arb::TableTurns turns{};
     const double multiplier = scaled_frequencies(who, *scaling, turns.value);
-    require(positions >= 0, who, "positions must not be negative");
+    require(positions >= 0 && positions <= 1 << 30, who, "positions must be 0..2^30");
     if (positions == 0) return AR_OK;
     require(cos_table != nullptr && sin_table != nullptr && aligned16(cos_table) && aligned16(sin_table), who,
             "the tables must be 16-byte aligned device arrays");

@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t item = 0;
     uint32_t segment = 0;
     do {
-      if (segment > 0 && !mbar_wait(smem_u32(&ctl.q_empty), (segment - 1) & 1, &ctl.abort)) {
+      if (segment > 0 && !mbar_wait_called(smem_u32(&ctl.q_empty), (segment - 1) & 1, &ctl.abort)) {
         ok = false;
         break;
       }
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv, ++item) {
           const uint32_t stage = stage_of(item);
-          if (item >= kStages && !mbar_wait(smem_u32(&ctl.empty[stage]), phase_of(item) ^ 1, &ctl.abort)) {
+          if (item >= kStages && !mbar_wait_called(smem_u32(&ctl.empty[stage]), phase_of(item) ^ 1, &ctl.abort)) {
             ok = false;
             break;
           }
@@ -331,9 +331,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         ctl.abort = 1;
       }
       // the loads in flight land before the shared memory is released
-      if (segment > 0) mbar_wait(smem_u32(&ctl.q_full), (segment - 1) & 1, nullptr);
+      if (segment > 0) mbar_wait_called(smem_u32(&ctl.q_full), (segment - 1) & 1, nullptr);
       for (uint32_t i = item > kStages ? item - kStages : 0; i < item; ++i) {
-        mbar_wait(smem_u32(&ctl.full[stage_of(i)]), phase_of(i), nullptr);
+        mbar_wait_called(smem_u32(&ctl.full[stage_of(i)]), phase_of(i), nullptr);
       }
     }
   } else if (warp == 9) {
@@ -371,11 +371,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       auto wait_k = [&](uint32_t n) {
-        const bool there = mbar_wait(smem_u32(&ctl.full[stage_of(2 * n)]), phase_of(2 * n), &ctl.abort);
+        const bool there = mbar_wait_called(smem_u32(&ctl.full[stage_of(2 * n)]), phase_of(2 * n), &ctl.abort);
         fence_after();
         return there;
       };
-      ok = mbar_wait(smem_u32(&ctl.q_full), segment & 1, &ctl.abort) && wait_k(turn);
+      ok = mbar_wait_called(smem_u32(&ctl.q_full), segment & 1, &ctl.abort) && wait_k(turn);
       if (!ok) break;
       scores(0, w.block, turn);
       scores(1, w.block, turn);
@@ -383,9 +383,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int b = w.block; ok && b < end; ++b, ++turn) {
         const uint32_t v_item = 2 * turn + 1;
         const uint32_t stage = stage_of(v_item);
-        ok = mbar_wait(smem_u32(&ctl.full[stage]), phase_of(v_item), &ctl.abort);
+        ok = mbar_wait_called(smem_u32(&ctl.full[stage]), phase_of(v_item), &ctl.abort);
         if (ok && !w.whole(b, window)) {  // V of this block is cleared by the softmax warps first
-          ok = mbar_wait(smem_u32(&ctl.clean[turn & 1]), (cleaned >> (turn & 1)) & 1, &ctl.abort);
+          ok = mbar_wait_called(smem_u32(&ctl.clean[turn & 1]), (cleaned >> (turn & 1)) & 1, &ctl.abort);
           cleaned ^= 1u << (turn & 1);
         }
         const uint64_t v_at = desc_mn_major(ring + stage * kOperand, kHalfBytes);
@@ -393,17 +393,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int half = 0; half < 2; ++half) {
           const bool needed = needs(half, b);
           if (ok && needed && !(waited_o >> half & 1)) {
-            ok = mbar_wait(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
+            ok = mbar_wait_called(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
             waited_o |= 1u << half;
           }
 #pragma unroll
           for (int part = 0; part < 2; ++part) {
-            ok = ok && mbar_wait(smem_u32(&ctl.p_full[half][part]), turn & 1, &ctl.abort);
+            ok = ok && mbar_wait_called(smem_u32(&ctl.p_full[half][part]), turn & 1, &ctl.abort);
             fence_after();
             if (ok && needed) {
               const bool first = b == (half == 0 ? begin0 : begin1);
 #pragma unroll
-              for (int k = part * 4; k < part * 4 + 4; ++k) {  // 16 keys a step
+              for (int k = part * 6; k < 6 + part * 2; ++k) {  // 16 keys a step
                 mma_ts(elected, tmem + kTmemO + half * 128, tmem + half * 128 + k * 8, v_at + k * (16 * 128 >> 4),
                        c.idesc_o, first && k == 0 ? 0u : 1u);
               }
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        if (ok && !(waited_o >> half & 1)) ok = mbar_wait(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
+        if (ok && !(waited_o >> half & 1)) ok = mbar_wait_called(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
         // a half without blocks takes part too, so that its softmax warps stay within a segment of it
         if (ok && (half == 0 ? begin0 == end0 : begin1 == end1)) mbar_arrive_if(elected, smem_u32(&ctl.o_full[half]));
       }
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // every MMA has completed before TMEM and shared memory are released
     mma_commit(elected, smem_u32(&ctl.done));
-    mbar_wait(smem_u32(&ctl.done), 0, nullptr);
+    mbar_wait_called(smem_u32(&ctl.done), 0, nullptr);
   } else {
     // --------------------------------------------------------------------------------- softmax
     const int half = warp >> 2;
@@ -466,14 +466,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int key0 = (w.tile.block_begin + b) * kChunkBlock;
         // every block passes through s_full and p_full, needed by the half or not, so that neither side
         // is ever more than one phase ahead of a barrier that it waits on
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl.s_full[half]), turn & 1, &ctl.abort));
+        ok = __all_sync(0xffffffffu, mbar_wait_called(smem_u32(&ctl.s_full[half]), turn & 1, &ctl.abort));
         if (!ok) break;
         if (!whole) {
           // Clear what no row of the tile sees, and values that are not finite (a probability of zero
           // times one would be NaN); the rows that see those get them added at the end.
           const uint32_t v_item = 2 * turn + 1;
           ok = __all_sync(0xffffffffu,
-                          mbar_wait(smem_u32(&ctl.full[stage_of(v_item)]), phase_of(v_item), &ctl.abort));
+                          mbar_wait_called(smem_u32(&ctl.full[stage_of(v_item)]), phase_of(v_item), &ctl.abort));
           if (!ok) break;
           uint4* v = reinterpret_cast<uint4*>(smem + Layout<kDim>::kRing + stage_of(v_item) * kOperand);
           bool bad = false;
@@ -509,32 +509,35 @@ __global__ void __launch_bounds__(kThreads, 1)
           continue;
         }
         fence_after();
-        // S passes through the registers 64 columns at a time, twice: the upper and the lower half for the
-        // maximum, the lower (still there) and the upper for the probabilities. P's 16-bit pairs take the
-        // place of scores already read.
+        // S passes through the registers twice, 32 columns a time: C D A B for the maximum, A B (still
+        // there) C D for the probabilities, whose loads hide behind the exponentials before them. P's
+        // 16-bit pairs take the place of scores already read. The products with V start when A B C are
+        // there, so that those of D alone stand between the last probability and the next scores.
         const int low = row_first - key0;
         const int high = row_last - key0;
-        float x[64];
-        auto load = [&](int column) {
-          uint32_t raw[2][32];
-          tmem_ld32(s_tmem + column, raw[0]);
-          tmem_ld32(s_tmem + column + 32, raw[1]);
-          tmem_wait_ld();
+        uint32_t x[2][32];
+        auto mask = [&](uint32_t (&v)[32], int column) {
+          if (__builtin_expect(whole, 1)) return;
 #pragma unroll
-          for (int i = 0; i < 64; ++i) x[i] = __uint_as_float(raw[i >> 5][i & 31]);
-          if (!whole) {
-#pragma unroll
-            for (int i = 0; i < 64; ++i) x[i] = i + column > high || i + column < low ? -INFINITY : x[i];
+          for (int i = 0; i < 32; ++i) {
+            if (i + column > high || i + column < low) v[i] = __float_as_uint(-INFINITY);
           }
         };
         float top[kChains];
 #pragma unroll
         for (int i = 0; i < kChains; ++i) top[i] = -INFINITY;
 #pragma unroll 1
-        for (int column = 0; column < kChunkBlock; column += 64) {
-          load(column);
+        for (int column = 64; column >= 0; column -= 64) {
+          tmem_ld32(s_tmem + column, x[0]);
+          tmem_ld32(s_tmem + column + 32, x[1]);
+          tmem_wait_ld();
+          mask(x[0], column);
+          mask(x[1], column + 32);
 #pragma unroll
-          for (int i = 0; i < 64; i += 2) top[(i / 2) % kChains] = max3(top[(i / 2) % kChains], x[i], x[i + 1]);
+          for (int i = 0; i < 64; i += 2) {
+            top[(i / 2) % kChains] = max3(top[(i / 2) % kChains], __uint_as_float(x[i >> 5][i & 31]),
+                                          __uint_as_float(x[i >> 5][(i & 31) + 1]));
+          }
         }
         const float block_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
         // the row's reference moves only when the block's maximum exceeds it by more than the threshold,
@@ -543,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool rescale = move && reference != -INFINITY;
         if (__any_sync(0xffffffffu, rescale)) {
           // O holds the segment's blocks before this one
-          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl.o_full[half]), (outputs - 1) & 1, &ctl.abort));
+          ok = __all_sync(0xffffffffu, mbar_wait_called(smem_u32(&ctl.o_full[half]), (outputs - 1) & 1, &ctl.abort));
           if (!ok) break;
           fence_after();
           const float factor = rescale ? ex2_ftz(reference - block_top) : 1.0f;
@@ -565,24 +568,45 @@ __global__ void __launch_bounds__(kThreads, 1)
         unsigned long long sums[kChains / 2];
 #pragma unroll
         for (int i = 0; i < kChains / 2; ++i) sums[i] = 0ull;
-#pragma unroll 1
-        for (int part = 0; part < 2; ++part) {
-          load(part * 64);
-          uint32_t packed[32];
+        auto probabilities = [&](const uint32_t (&v)[32], uint32_t column) {
+          uint32_t packed[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
+          for (int i = 0; i < 16; ++i) {
             float p0, p1;
-            unpack_f32x2(fma_f32x2(pack_f32x2(x[2 * i], x[2 * i + 1]), scale2, base2), p0, p1);
+            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale2, base2),
+                         p0, p1);
             p0 = ex2_ftz(p0);
             p1 = ex2_ftz(p1);
             sums[i % (kChains / 2)] = add_f32x2(sums[i % (kChains / 2)], pack_f32x2(p0, p1));
             packed[i] = pack2<T>(p0, p1);
           }
-          tmem_st32(s_tmem + part * 32, packed);
-          tmem_wait_st();
-          fence_before();
-          mbar_arrive_if(elected, smem_u32(&ctl.p_full[half][part]));
+          tmem_st16(s_tmem + column, packed);
+        };
+        // Rolled: the softmax and MMA warps of an SM quarter share an instruction cache that the unrolled
+        // form does not fit (886 against 846 us for two 4K chunks; a quarter of the exponentials as
+        // polynomials on the FMA pipe: 846 against 864 us, the same within the noise, and left out).
+#pragma unroll 1
+        for (int pair = 0; pair < 2; ++pair) {
+          probabilities(x[0], pair * 32);
+          if (pair == 0) {
+            tmem_ld32(s_tmem + 64, x[0]);
+          } else {
+            tmem_wait_st();
+            fence_before();
+            mbar_arrive_if(elected, smem_u32(&ctl.p_full[half][0]));
+            tmem_wait_ld();
+            mask(x[1], 96);
+          }
+          probabilities(x[1], pair * 32 + 16);
+          if (pair == 0) {
+            tmem_wait_ld();
+            tmem_ld32(s_tmem + 96, x[1]);
+            mask(x[0], 64);
+          }
         }
+        tmem_wait_st();
+        fence_before();
+        mbar_arrive_if(elected, smem_u32(&ctl.p_full[half][1]));
 #pragma unroll
         for (int i = 0; i < kChains / 2; ++i) {
           float s0, s1;
@@ -595,14 +619,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---- the segment's rows: O / l, or the partial sums
       const bool any = h_end > h_begin;
       if (!any) ++outputs;
-      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl.o_full[half]), (outputs - 1) & 1, &ctl.abort));
+      ok = __all_sync(0xffffffffu, mbar_wait_called(smem_u32(&ctl.o_full[half]), (outputs - 1) & 1, &ctl.abort));
       if (!ok) break;
       fence_after();
       // every thread's share of the cleared blocks is done when their barriers' last phases are
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if ((cleaned_once >> i & 1) && ok) {
-          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl.clean[i]), ((cleaned >> i) & 1) ^ 1, &ctl.abort));
+          ok = __all_sync(0xffffffffu, mbar_wait_called(smem_u32(&ctl.clean[i]), ((cleaned >> i) & 1) ^ 1, &ctl.abort));
         }
       }
       if (!ok) break;

@@ -321,7 +321,7 @@ int ar_decode_attention(const void* q, const void* k_cache, const void* v_cache,
  *                   b = min(ceil(c(low)), r - 1), g = clamp((i - a) / max(b - a, 0.001), 0, 1):
  *                   g f_i / s + (1 - g) f_i; cos and sin are multiplied by 0.1 ln(s) + 1.
  * attention_factor, where it is not 0, replaces that multiplier (1 for the other kinds).
- * theta > 1, finite; rotary_dim even, 2..512; for LINEAR, BANDS and YARN s >= 1; for BANDS and
+ * theta > 1, finite; rotary_dim even, 2..512; at most 2^30 positions; for LINEAR, BANDS and YARN s >= 1; for BANDS and
  * YARN L >= 1 and 0 < low < high. */
 #define AR_ROPE_NONE 0
 #define AR_ROPE_LINEAR 1
