@@ -77,6 +77,14 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t phase, const vo
 static __device__ __noinline__ bool mbar_wait_loop(uint32_t bar, uint32_t phase, const volatile int* abort) {
   return mbar_wait(bar, phase, abort);
 }
+// The wait of a role that carries on when it gives up: it reports the timeout and sets *abort, after
+// which every such wait returns at once and the rest of the work runs through on what is there.
+static __device__ __noinline__ void mbar_wait_or_abort(uint32_t bar, uint32_t phase, volatile int* abort, int* status) {
+  if (*abort) return;
+  if (mbar_wait(bar, phase, abort)) return;
+  report_status(status, kStatusWaitTimeout);
+  *abort = 1;
+}
 __device__ __forceinline__ bool mbar_wait_called(uint32_t bar, uint32_t phase, const volatile int* abort) {
   return mbar_try(bar, phase) || mbar_wait_loop(bar, phase, abort);
 }

@@ -20,8 +20,8 @@
 // kernel adds up in order.
 // Masked rows and positions: scores by selection; V values that not every row may see, by clearing the
 // tile's copy (slots past the end, values that are not finite) before the product.
-// Every mbarrier wait is bounded; on expiry the kernel records kStatusWaitTimeout, waits (bounded) for
-// its own MMAs and copies, frees TMEM and returns.
+// Every mbarrier wait is bounded; on expiry the kernel records kStatusWaitTimeout, loads no more, runs
+// through the rest without waiting, waits (bounded) for its own MMAs and copies, frees TMEM and returns.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -266,10 +266,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Ring item 2n is K of the part's n-th block, item 2n + 1 its V: stage item % 4, phase item / 4.
   auto stage_of = [](uint32_t item) { return item % kStages; };
   auto phase_of = [](uint32_t item) { return (item / kStages) & 1; };
-  bool ok = true;
+  auto wait = [&](uint64_t& bar, uint32_t phase) {
+    if (!mbar_try(smem_u32(&bar), phase)) mbar_wait_or_abort(smem_u32(&bar), phase, &ctl.abort, a.status);
+    __syncwarp();
+  };
 
   if (warp == 8) {
     // ------------------------------------------------------------------------------------- TMA
+    bool ok = true;
     const int page_rows = min(1 << a.cache.page_shift, kChunkBlock);
     const int boxes = kChunkBlock / page_rows * kHalves;
     const int my_page = lane / kHalves;  // the lane's box: page and 64-wide half
@@ -371,36 +375,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       auto wait_k = [&](uint32_t n) {
-        const bool there = mbar_wait_called(smem_u32(&ctl.full[stage_of(2 * n)]), phase_of(2 * n), &ctl.abort);
+        wait(ctl.full[stage_of(2 * n)], phase_of(2 * n));
         fence_after();
-        return there;
       };
-      ok = mbar_wait_called(smem_u32(&ctl.q_full), segment & 1, &ctl.abort) && wait_k(turn);
-      if (!ok) break;
+      wait(ctl.q_full, segment & 1);
+      wait_k(turn);
       scores(0, w.block, turn);
       scores(1, w.block, turn);
       uint32_t waited_o = segment == 0 ? 3u : 0u;  // halves whose O of the last segment has been read
-      for (int b = w.block; ok && b < end; ++b, ++turn) {
+      for (int b = w.block; b < end; ++b, ++turn) {
         const uint32_t v_item = 2 * turn + 1;
         const uint32_t stage = stage_of(v_item);
-        ok = mbar_wait_called(smem_u32(&ctl.full[stage]), phase_of(v_item), &ctl.abort);
-        if (ok && !w.whole(b, window)) {  // V of this block is cleared by the softmax warps first
-          ok = mbar_wait_called(smem_u32(&ctl.clean[turn & 1]), (cleaned >> (turn & 1)) & 1, &ctl.abort);
+        wait(ctl.full[stage], phase_of(v_item));
+        if (!w.whole(b, window)) {  // V of this block is cleared by the softmax warps first
+          wait(ctl.clean[turn & 1], (cleaned >> (turn & 1)) & 1);
           cleaned ^= 1u << (turn & 1);
         }
         const uint64_t v_at = desc_mn_major(ring + stage * kOperand, kHalfBytes);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const bool needed = needs(half, b);
-          if (ok && needed && !(waited_o >> half & 1)) {
-            ok = mbar_wait_called(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
+          if (needed && !(waited_o >> half & 1)) {
+            wait(ctl.o_free[half], (segment - 1) & 1);
             waited_o |= 1u << half;
           }
 #pragma unroll
           for (int part = 0; part < 2; ++part) {
-            ok = ok && mbar_wait_called(smem_u32(&ctl.p_full[half][part]), turn & 1, &ctl.abort);
+            // a wait behind MMAs stalls until they have drained, so the next K is waited for up here
+            if (half == 0 && part == 1 && b + 1 < end) wait_k(turn + 1);
+            wait(ctl.p_full[half][part], turn & 1);
             fence_after();
-            if (ok && needed) {
+            if (needed) {
               const bool first = b == (half == 0 ? begin0 : begin1);
 #pragma unroll
               for (int k = part * 6; k < 6 + part * 2; ++k) {  // 16 keys a step
@@ -410,25 +415,18 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (part == 1) mma_commit(elected, smem_u32(&ctl.o_full[half]));
             }
           }
-          if (ok && half == 1) mma_commit(elected, smem_u32(&ctl.empty[stage]));
-          if (ok && b + 1 < end) {
-            if (half == 0) ok = wait_k(turn + 1);
-            if (ok) scores(half, b + 1, turn + 1);
-          }
+          if (half == 1) mma_commit(elected, smem_u32(&ctl.empty[stage]));
+          if (b + 1 < end) scores(half, b + 1, turn + 1);
         }
       }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        if (ok && !(waited_o >> half & 1)) ok = mbar_wait_called(smem_u32(&ctl.o_free[half]), (segment - 1) & 1, &ctl.abort);
+        if (!(waited_o >> half & 1)) wait(ctl.o_free[half], (segment - 1) & 1);
         // a half without blocks takes part too, so that its softmax warps stay within a segment of it
-        if (ok && (half == 0 ? begin0 == end0 : begin1 == end1)) mbar_arrive_if(elected, smem_u32(&ctl.o_full[half]));
+        if ((half == 0 ? begin0 == end0 : begin1 == end1)) mbar_arrive_if(elected, smem_u32(&ctl.o_full[half]));
       }
       ++segment;
-    } while (ok && walk_next(w, c));
-    if (!ok && lane == 0) {
-      report_status(a.status, kStatusWaitTimeout);
-      ctl.abort = 1;
-    }
+    } while (walk_next(w, c));
     // every MMA has completed before TMEM and shared memory are released
     mma_commit(elected, smem_u32(&ctl.done));
     mbar_wait_called(smem_u32(&ctl.done), 0, nullptr);
@@ -466,15 +464,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int key0 = (w.tile.block_begin + b) * kChunkBlock;
         // every block passes through s_full and p_full, needed by the half or not, so that neither side
         // is ever more than one phase ahead of a barrier that it waits on
-        ok = __all_sync(0xffffffffu, mbar_wait_called(smem_u32(&ctl.s_full[half]), turn & 1, &ctl.abort));
-        if (!ok) break;
+        wait(ctl.s_full[half], turn & 1);
         if (!whole) {
           // Clear what no row of the tile sees, and values that are not finite (a probability of zero
           // times one would be NaN); the rows that see those get them added at the end.
           const uint32_t v_item = 2 * turn + 1;
-          ok = __all_sync(0xffffffffu,
-                          mbar_wait_called(smem_u32(&ctl.full[stage_of(v_item)]), phase_of(v_item), &ctl.abort));
-          if (!ok) break;
+          wait(ctl.full[stage_of(v_item)], phase_of(v_item));
           uint4* v = reinterpret_cast<uint4*>(smem + Layout<kDim>::kRing + stage_of(v_item) * kOperand);
           bool bad = false;
 #pragma unroll 4
@@ -546,8 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool rescale = move && reference != -INFINITY;
         if (__any_sync(0xffffffffu, rescale)) {
           // O holds the segment's blocks before this one
-          ok = __all_sync(0xffffffffu, mbar_wait_called(smem_u32(&ctl.o_full[half]), (outputs - 1) & 1, &ctl.abort));
-          if (!ok) break;
+          wait(ctl.o_full[half], (outputs - 1) & 1);
           fence_after();
           const float factor = rescale ? ex2_ftz(reference - block_top) : 1.0f;
 #pragma unroll 1
@@ -615,21 +609,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ++outputs;
       }
-      if (!ok) break;
       // ---- the segment's rows: O / l, or the partial sums
       const bool any = h_end > h_begin;
       if (!any) ++outputs;
-      ok = __all_sync(0xffffffffu, mbar_wait_called(smem_u32(&ctl.o_full[half]), (outputs - 1) & 1, &ctl.abort));
-      if (!ok) break;
+      wait(ctl.o_full[half], (outputs - 1) & 1);
       fence_after();
       // every thread's share of the cleared blocks is done when their barriers' last phases are
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if ((cleaned_once >> i & 1) && ok) {
-          ok = __all_sync(0xffffffffu, mbar_wait_called(smem_u32(&ctl.clean[i]), ((cleaned >> i) & 1) ^ 1, &ctl.abort));
-        }
+        if (cleaned_once >> i & 1) wait(ctl.clean[i], ((cleaned >> i) & 1) ^ 1);
       }
-      if (!ok) break;
       const bool poisoned = (*reinterpret_cast<volatile unsigned*>(&ctl.poison) >> (segment & 31)) & 1;
       const bool begins = w.block == 0;
       const bool complete = begins && w.count == w.tile.blocks;
@@ -689,10 +678,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       ++segment;
     } while (walk_next(w, c));
-    if (!ok && lane == 0) {
-      report_status(a.status, kStatusWaitTimeout);
-      ctl.abort = 1;
-    }
   }
 
   __syncwarp();
