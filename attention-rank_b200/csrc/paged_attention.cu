@@ -5,7 +5,7 @@
 // over the visible positions, in one pass with a running reference m and sum.
 //
 // Few rows a KV head (single tokens, a few drafted ones: at most 32 rows of new tokens x query heads
-// of the group): every K and V value is used once per call, so HBM bounds the kernel. K and V arrive
+// of the group): every K and V value is used once or twice per call, so HBM bounds the kernel. K and V arrive
 // in 64-key blocks by TMA (192 KB of ring per SM, above the 45 KB that 6.5 TB/s x 1 us of latency
 // needs), and the products run on mma.sync m16n8k16 with the group's rows as its 16 rows: the 128 rows
 // of a tcgen05 tile would be 7/8 empty.
@@ -32,16 +32,22 @@ namespace {
 using namespace async;
 
 constexpr int kBlock = 64;          // keys a block
+constexpr int kRows = 16;           // rows a tile
 constexpr int kCombineThreads = 256;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 
-// One (sequence, KV head) of the line of work.
+// One (sequence, KV head, 16 rows) of the line of work.
 struct FewTile {
   int first_position;  // of the first new token; negative when fewer are cached than new
   int first_key;       // smallest key any row sees (0 when none)
   int block_begin;     // key blocks [block_begin, block_begin + blocks)
   int blocks;          // at least 1
 };
+
+// 16-row tiles of a sequence's rows, new tokens x query heads of a KV head.
+__device__ __forceinline__ int few_row_tiles(const PagedAttentionArgs& a, const PagedSequence& seq) {
+  return (seq.q_len * (a.query_heads / a.cache.kv_heads) + kRows - 1) / kRows;
+}
 
 __device__ __forceinline__ FewTile few_tile(const PagedSequence& seq, int window) {
   FewTile t;
@@ -55,27 +61,26 @@ __device__ __forceinline__ FewTile few_tile(const PagedSequence& seq, int window
 // Units of a sequence; 0 without new tokens, or with more of them than this form takes.
 __device__ __forceinline__ int64_t few_units(const PagedAttentionArgs& a, const PagedSequence& seq, int most) {
   if (seq.q_len == 0 || seq.q_len > most) return 0;
-  return static_cast<int64_t>(few_tile(seq, a.sliding_window).blocks) * a.cache.kv_heads;
+  return static_cast<int64_t>(few_tile(seq, a.sliding_window).blocks) * few_row_tiles(a, seq) * a.cache.kv_heads;
 }
 
-// A CTA has kGroups groups of four warps, a group for each 16 rows; they read the same blocks. One
-// group: two CTAs an SM with three stages each; two: one CTA with six (its 128 accumulators a thread
-// and the query operands of 32 rows would not fit four warps' registers).
-template <int kGroups, int kDim>
+// Two CTAs an SM, three stages each. A sequence of 17 to 32 rows is two tiles, whose second reading of K
+// and V comes from L2: one CTA of eight consumer warps for both tiles, with six stages, had too few
+// warps to hide its chains behind (RT_TIMES).
+template <int kDim>
 struct FewShared {
-  static constexpr int kThreads = (4 * kGroups + 1) * 32;
-  static constexpr int kCtasPerSm = kGroups == 1 ? 2 : 1;
-  static constexpr int kStages = kGroups == 1 ? 3 : 6;
-  static constexpr int kRows = 16 * kGroups;
+  static constexpr int kThreads = 5 * 32;
+  static constexpr int kCtasPerSm = 2;
+  static constexpr int kStages = 3;
   static constexpr uint32_t kBlockBytes = kBlock * kDim * 2;  // of K, or of V
   static constexpr int kPad = 36;                             // floats a merge row of 32 takes
   uint64_t full[kStages];
   uint64_t empty[kStages];
   volatile int abort;
-  int poison[kGroups][2];  // of this segment and the next, in turn
+  int poison[2];  // of this segment and the next, in turn
   PlanScratch<kThreads> plan;
-  float2 stats[kGroups][4][16];
-  alignas(16) float merge[kGroups][4][16][kPad];
+  float2 stats[4][kRows];
+  alignas(16) float merge[4][kRows][kPad];
   static constexpr size_t bytes() { return 2 * kStages * kBlockBytes + sizeof(FewShared) + 1024; }
 };
 
@@ -107,13 +112,7 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
   }
 }
 
-__device__ __forceinline__ void group_barrier(int group) {
-  if (group == 0) {
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-  } else {
-    asm volatile("bar.sync 2, 128;" ::: "memory");
-  }
-}
+__device__ __forceinline__ void consumer_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 template <typename T>
 __device__ __forceinline__ bool nonfinite_half(uint32_t bits) {
@@ -149,14 +148,13 @@ __device__ float nonfinite_sum(const PagedAttentionArgs& a, int s, int kv_head, 
   return sum;
 }
 
-template <typename T, int kGroups, int kDim>
-__global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<kGroups, kDim>::kCtasPerSm)
+template <typename T, int kDim>
+__global__ void __launch_bounds__(FewShared<kDim>::kThreads, FewShared<kDim>::kCtasPerSm)
     paged_attention_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                                const __grid_constant__ PagedAttentionArgs a, int most) {
-  using Shared = FewShared<kGroups, kDim>;
+  using Shared = FewShared<kDim>;
   constexpr int kThreads = Shared::kThreads;
   constexpr int kStages = Shared::kStages;
-  constexpr int kRows = Shared::kRows;
   constexpr uint32_t kBlockBytes = Shared::kBlockBytes;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -169,10 +167,10 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(smem_u32(&sh.full[i]), 1);
-      mbar_init(smem_u32(&sh.empty[i]), 4 * kGroups);
+      mbar_init(smem_u32(&sh.empty[i]), 4);
     }
     sh.abort = 0;
-    for (int i = 0; i < kGroups; ++i) sh.poison[i][0] = sh.poison[i][1] = 0;
+    sh.poison[0] = sh.poison[1] = 0;
     mbar_init_fence();
     prefetch_map(&k_map);
     prefetch_map(&v_map);
@@ -194,25 +192,31 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
   PagedSequence seq = place.seq;
   FewTile tile = few_tile(seq, a.sliding_window);
   const int64_t begin = place.cut.begin(blockIdx.x);
-  int kv_head = static_cast<int>(PlanCut::divide(begin - place.before, tile.blocks));
-  int block = static_cast<int>(begin - place.before - static_cast<int64_t>(kv_head) * tile.blocks);
+  int row_tiles = few_row_tiles(a, seq);
+  const int first_tile = static_cast<int>(PlanCut::divide(begin - place.before, tile.blocks));
+  int kv_head = first_tile / row_tiles;
+  int row_tile = first_tile - kv_head * row_tiles;
+  int block = static_cast<int>(begin - place.before - static_cast<int64_t>(first_tile) * tile.blocks);
   int64_t left = place.cut.begin(blockIdx.x + 1) - begin;
-  if (tid == 0) leave_join_tile(partials.tiles, &place, 0, kv_head, begin - block, tile.blocks);
+  if (tid == 0) leave_join_tile(partials.tiles, &place, row_tile, kv_head, begin - block, tile.blocks);
   auto next_tile = [&] {
     block = 0;
+    if (++row_tile < row_tiles) return;
+    row_tile = 0;
     if (++kv_head < a.cache.kv_heads) return;
     kv_head = 0;
     do {  // `left` units remain, so a sequence with new tokens follows
       seq = paged_sequence(a.batch, ++s, nullptr);
     } while (few_units(a, seq, most) == 0 && s + 1 < a.batch.sequences);
     tile = few_tile(seq, a.sliding_window);
+    row_tiles = few_row_tiles(a, seq);
   };
 
   const int page_rows = min(1 << a.cache.page_shift, kBlock);  // rows of one TMA box
   const int boxes = kBlock / page_rows;
   uint32_t turn = 0;  // blocks done so far: stage turn % kStages, phase turn / kStages
 
-  if (warp == 4 * kGroups) {
+  if (warp == 4) {
     // ---------------------------------------------------------------------------------- producer
     bool ok = true;
     while (ok && left > 0) {
@@ -262,8 +266,7 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
 
   // ------------------------------------------------------------------------------------ consumers
   const int group = a.query_heads / a.cache.kv_heads;
-  const int part16 = warp >> 2;  // the warp's group of 16 rows
-  const int quarter = warp & 3;  // its 16 keys of a block
+  const int quarter = warp;  // the warp's 16 keys of a block
   const int g = lane >> 2;
   const int t4 = lane & 3;
   // this lane's addresses inside a block: [page][64-wide half][row][128 bytes], 16-byte chunks XORed
@@ -293,7 +296,7 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
     int first_key[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int row = part16 * 16 + e * 8 + g;
+      const int row = row_tile * kRows + e * 8 + g;
       const int token = row / group;
       const bool in = row < rows;
       last_key[e] = in ? tile.first_position + token : -1;
@@ -418,27 +421,27 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
     if (!ok) break;
 
     // ---- join the four warps' sums: common reference, then 32 columns at a time through shared memory
-    if (__any_sync(0xffffffffu, poison) && lane == 0) sh.poison[part16][segment & 1] = 1;
+    if (__any_sync(0xffffffffu, poison) && lane == 0) sh.poison[segment & 1] = 1;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-      if (t4 == 0) sh.stats[part16][quarter][e * 8 + g] = make_float2(reference[e], l[e]);
+      if (t4 == 0) sh.stats[quarter][e * 8 + g] = make_float2(reference[e], l[e]);
     }
-    group_barrier(part16);
-    const bool poisoned = sh.poison[part16][segment & 1] != 0;
+    consumer_barrier();
+    const bool poisoned = sh.poison[segment & 1] != 0;
     // the other flag's readers have passed the last segment's barriers
-    if (quarter == 0 && lane == 0) sh.poison[part16][(segment + 1) & 1] = 0;
+    if (quarter == 0 && lane == 0) sh.poison[(segment + 1) & 1] = 0;
     const bool begins = block == 0;
     const bool complete = begins && count == tile.blocks;
     const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (begins ? 1 : 0);
     auto joined = [&](int row) {  // (reference, sum) of one of the 16 rows over the warps
       float2 all = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) all.x = fmaxf(all.x, sh.stats[part16][w][row].x);
+      for (int w = 0; w < 4; ++w) all.x = fmaxf(all.x, sh.stats[w][row].x);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const float2 part = sh.stats[part16][w][row];
+        const float2 part = sh.stats[w][row];
         all.y += part.y * (part.x == -INFINITY ? 0.0f : ex2_ftz(part.x - all.x));
       }
       return all;
@@ -454,7 +457,7 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
     }
     // this thread's place in a pass: 16 rows x 32 columns, four columns a thread
     const int merge_row = quarter * 4 + (lane >> 3);
-    const int row = part16 * 16 + merge_row;
+    const int row = row_tile * kRows + merge_row;
     const int token = row / group;
     const int head = kv_head * group + row - token * group;
     const float2 all = joined(merge_row);
@@ -465,17 +468,17 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
       for (int d = 0; d < 4; ++d) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          *reinterpret_cast<float2*>(&sh.merge[part16][quarter][e * 8 + g][d * 8 + 2 * t4]) =
+          *reinterpret_cast<float2*>(&sh.merge[quarter][e * 8 + g][d * 8 + 2 * t4]) =
               make_float2(o[4 * c + d][2 * e], o[4 * c + d][2 * e + 1]);
         }
       }
-      group_barrier(part16);
+      consumer_barrier();
       if (row < rows) {
         const int column = c * 32 + (lane & 7) * 4;
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const float4 part = *reinterpret_cast<const float4*>(&sh.merge[part16][w][merge_row][(lane & 7) * 4]);
+          const float4 part = *reinterpret_cast<const float4*>(&sh.merge[w][merge_row][(lane & 7) * 4]);
           sum.x += part.x;
           sum.y += part.y;
           sum.z += part.z;
@@ -500,11 +503,11 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
                 all.y != 0.0f ? all.x + log2f(all.y) : -INFINITY;
           }
         } else {
-          *reinterpret_cast<float4*>(partials.sums + (slot * kRows + row) * kDim + column) = sum;
-          if (column == 0) partials.stats[slot * kRows + row] = all;
+          *reinterpret_cast<float4*>(partials.sums + (slot * kRows + merge_row) * kDim + column) = sum;
+          if (column == 0) partials.stats[slot * kRows + merge_row] = all;
         }
       }
-      group_barrier(part16);
+      consumer_barrier();
     }
     ++segment;
     left -= count;
@@ -517,7 +520,7 @@ __global__ void __launch_bounds__(FewShared<kGroups, kDim>::kThreads, FewShared<
 }
 
 // Joins the parts of the tile that the beginning of part blockIdx.x + 1 cuts, in the order of the CTAs.
-template <typename T, int kRows, int kDim>
+template <typename T, int kDim>
 __global__ void __launch_bounds__(kCombineThreads) paged_attention_few_join_kernel(const PagedAttentionArgs a, int ctas) {
   // every thread waits, so that this grid does not complete before the one whose sums it reads
   wait_for_producer();
@@ -530,7 +533,7 @@ __global__ void __launch_bounds__(kCombineThreads) paged_attention_few_join_kern
   const int kv_head = join.kv_head;
   const int c = blockIdx.x;  // the part in which the tile begins
   const int group = a.query_heads / a.cache.kv_heads;
-  const int rows = seq.q_len * group;
+  const int rows = min(kRows, seq.q_len * group - join.tile * kRows);  // of the tile
   constexpr int kBatch = 8;  // parts whose loads are in flight together
   for (int item = blockIdx.y * kCombineThreads + threadIdx.x; item < rows * (kDim / 4);
        item += gridDim.y * kCombineThreads) {
@@ -573,8 +576,9 @@ __global__ void __launch_bounds__(kCombineThreads) paged_attention_few_join_kern
       }
     }
     const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
-    const int token = row / group;
-    const int head = kv_head * group + row - token * group;
+    const int seq_row = join.tile * kRows + row;
+    const int token = seq_row / group;
+    const int head = kv_head * group + seq_row - token * group;
     T* to = static_cast<T*>(a.out) + (seq.q_begin + token) * a.out_stride + head * kDim + column;
     *reinterpret_cast<uint2*>(to) =
         make_uint2(pack2<T>(o.x * inverse, o.y * inverse), pack2<T>(o.z * inverse, o.w * inverse));
@@ -603,22 +607,19 @@ bool encode_pages(CUtensorMap* map, const PagedCache& c, void* pages, int rows) 
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int kGroups>
-int few_ctas() {
-  return sm_count() * FewShared<kGroups, 128>::kCtasPerSm;
-}
+int few_ctas() { return sm_count() * FewShared<128>::kCtasPerSm; }
 
 // Takes the sequences of at most `most` new tokens.
-template <typename T, int kGroups, int kDim>
+template <typename T, int kDim>
 cudaError_t launch_few(const PagedAttentionArgs& a, int most, cudaStream_t stream) {
-  using Shared = FewShared<kGroups, kDim>;
+  using Shared = FewShared<kDim>;
   static_assert(Shared::kCtasPerSm * (Shared::bytes() + 1024) <= 228 * 1024, "the CTAs of an SM share its shared memory");
   int device = 0;
   cudaGetDevice(&device);
   static uint64_t configured = 0;  // the shared-memory opt-in is a per-device attribute
   if (device >= 64 || !(configured & (1ull << device))) {
     const cudaError_t status =
-        cudaFuncSetAttribute(paged_attention_few_kernel<T, kGroups, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        cudaFuncSetAttribute(paged_attention_few_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(Shared::bytes()));
     if (status != cudaSuccess) return status;
     if (device < 64) configured |= 1ull << device;
@@ -629,36 +630,32 @@ cudaError_t launch_few(const PagedAttentionArgs& a, int most, cudaStream_t strea
       !encode_pages<T>(&v_map, a.cache, a.cache.v_pages, rows)) {
     return cudaErrorInvalidValue;
   }
-  const int ctas = few_ctas<kGroups>();
-  const cudaError_t status = launch_overlapped(paged_attention_few_kernel<T, kGroups, kDim>, dim3(ctas),
+  const int ctas = few_ctas();
+  const cudaError_t status = launch_overlapped(paged_attention_few_kernel<T, kDim>, dim3(ctas),
                                                dim3(Shared::kThreads), Shared::bytes(), stream, k_map, v_map, a, most);
   if (status != cudaSuccess || ctas < 2) return status;
-  return launch_overlapped(paged_attention_few_join_kernel<T, Shared::kRows, kDim>, dim3(ctas - 1, Shared::kRows / 8),
+  return launch_overlapped(paged_attention_few_join_kernel<T, kDim>, dim3(ctas - 1, kRows / 8),
                            dim3(kCombineThreads), 0, stream, a, ctas);
 }
 
 // Which forms a batch takes. A sequence's rows are its new tokens times the query heads of a KV head.
-// Where no sequence has more than 32 rows the kernel of this file takes them all. Else the chunk kernel
-// takes them, except that in a batch of several sequences those of at most 16 rows go to this kernel
-// first, which reads the cache at HBM's rate where a 256-row tile of the other would be nearly empty
-// (13 single tokens and 6 chunks: CHOICE_TIMES).
+// Sequences of at most kFewRows rows go to the kernel of this file, which reads the cache at HBM's rate
+// where a 256-row tile of the chunk kernel would be nearly empty; the others to the chunk kernel. Only
+// what the bound on the new tokens allows for is launched, and a batch of one sequence with a larger
+// bound takes the chunk kernel alone: the launches it would save cost more than a short chunk there.
+// FORM_TIMES
+constexpr int kFewRows = 32;
+
 struct FormChoice {
-  int few_rows = 0;    // 16, 32, or 0: the few-row form is not launched
-  int few_tokens = 0;  // new tokens up to which a sequence takes it
+  int few_tokens = 0;  // new tokens up to which a sequence takes the few-row form; 0: not launched
   bool chunk = false;  // is the chunk form launched?
 };
 
 FormChoice choose_forms(const PagedCache& cache, const PagedBatch& batch, int query_heads) {
   const int group = query_heads / cache.kv_heads;
-  const int64_t rows = static_cast<int64_t>(batch.max_query) * group;
   FormChoice choice;
-  choice.chunk = rows > 32;
-  if (!choice.chunk) {
-    choice.few_rows = rows <= 16 ? 16 : 32;
-  } else if (batch.sequences > 1 && group <= 16) {
-    choice.few_rows = 16;
-  }
-  choice.few_tokens = choice.few_rows / group;
+  choice.chunk = static_cast<int64_t>(batch.max_query) * group > kFewRows;
+  if (!choice.chunk || batch.sequences > 1) choice.few_tokens = kFewRows / group;
   return choice;
 }
 
@@ -666,8 +663,7 @@ template <typename T, int kDim>
 cudaError_t launch_dim(const PagedAttentionArgs& a, cudaStream_t stream) {
   const FormChoice choice = choose_forms(a.cache, a.batch, a.query_heads);
   cudaError_t status = cudaSuccess;
-  if (choice.few_rows == 16) status = launch_few<T, 1, kDim>(a, choice.few_tokens, stream);
-  if (choice.few_rows == 32) status = launch_few<T, 2, kDim>(a, choice.few_tokens, stream);
+  if (choice.few_tokens > 0) status = launch_few<T, kDim>(a, choice.few_tokens, stream);
   if (status != cudaSuccess || !choice.chunk) return status;
   // the two forms' partial sums share the workspace: each kernel waits for the one before it
   return launch_paged_attention_chunk(a, choice.few_tokens, stream);
@@ -678,8 +674,7 @@ cudaError_t launch_dim(const PagedAttentionArgs& a, cudaStream_t stream) {
 int64_t paged_attention_workspace(const PagedCache& cache, const PagedBatch& batch, int query_heads) {
   const FormChoice choice = choose_forms(cache, batch, query_heads);
   int64_t bytes = choice.chunk ? paged_attention_chunk_workspace(cache.head_dim) : 0;
-  if (choice.few_rows == 16) bytes = std::max(bytes, partial_bytes(16, cache.head_dim, few_ctas<1>()));
-  if (choice.few_rows == 32) bytes = std::max(bytes, partial_bytes(32, cache.head_dim, few_ctas<2>()));
+  if (choice.few_tokens > 0) bytes = std::max(bytes, partial_bytes(kRows, cache.head_dim, few_ctas()));
   return bytes;
 }
 
