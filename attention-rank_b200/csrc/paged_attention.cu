@@ -4,8 +4,9 @@
 //   lse = m + log2 sum_j 2^(x_j - m),
 // over the visible positions, in one pass with a running reference m and sum.
 //
-// Few rows a KV head (single tokens, a few drafted ones: at most 32 rows of new tokens x query heads
-// of the group): every K and V value is used once or twice per call, so HBM bounds the kernel. K and V arrive
+// Few rows a KV head (single tokens, a few drafted ones: at most 48 rows of new tokens x query heads
+// of the group): every K and V value is used once to three times per call, so HBM bounds the kernel (64
+// single tokens over up to 8K keys, 1.24 GB: 191 us, 0.98 of the measured copy). K and V arrive
 // in 64-key blocks by TMA (192 KB of ring per SM, above the 45 KB that 6.5 TB/s x 1 us of latency
 // needs), and the products run on mma.sync m16n8k16 with the group's rows as its 16 rows: the 128 rows
 // of a tcgen05 tile would be 7/8 empty.
@@ -49,10 +50,15 @@ __device__ __forceinline__ int few_row_tiles(const PagedAttentionArgs& a, const 
   return (seq.q_len * (a.query_heads / a.cache.kv_heads) + kRows - 1) / kRows;
 }
 
+// Smallest key that the row at `position` sees; the window may be as large as an int gets.
+__device__ __forceinline__ int first_visible(int position, int window) {
+  return window > 0 && position >= window ? position - window + 1 : 0;
+}
+
 __device__ __forceinline__ FewTile few_tile(const PagedSequence& seq, int window) {
   FewTile t;
   t.first_position = seq.kv_len - seq.q_len;
-  t.first_key = window > 0 ? max(0, t.first_position - window + 1) : 0;
+  t.first_key = first_visible(t.first_position, window);
   t.block_begin = t.first_key / kBlock;
   t.blocks = max(1, (seq.kv_len + kBlock - 1) / kBlock - t.block_begin);
   return t;
@@ -64,9 +70,9 @@ __device__ __forceinline__ int64_t few_units(const PagedAttentionArgs& a, const 
   return static_cast<int64_t>(few_tile(seq, a.sliding_window).blocks) * few_row_tiles(a, seq) * a.cache.kv_heads;
 }
 
-// Two CTAs an SM, three stages each. A sequence of 17 to 32 rows is two tiles, whose second reading of K
-// and V comes from L2: one CTA of eight consumer warps for both tiles, with six stages, had too few
-// warps to hide its chains behind (RT_TIMES).
+// Two CTAs an SM, three stages each. A sequence of 17 rows and more is two or three tiles, whose later
+// readings of K and V come from L2: one CTA of eight consumer warps for both tiles, with six stages, had too few
+// warps to hide its chains behind (28 rows, 16 sequences over up to 4K keys: 28.3 against 33.0 us).
 template <int kDim>
 struct FewShared {
   static constexpr int kThreads = 5 * 32;
@@ -300,13 +306,13 @@ __global__ void __launch_bounds__(FewShared<kDim>::kThreads, FewShared<kDim>::kC
       const int token = row / group;
       const bool in = row < rows;
       last_key[e] = in ? tile.first_position + token : -1;
-      first_key[e] = a.sliding_window > 0 ? max(0, tile.first_position + token - a.sliding_window + 1) : 0;
+      first_key[e] = first_visible(tile.first_position + token, a.sliding_window);
       const T* from = static_cast<const T*>(a.q) + (seq.q_begin + (in ? token : 0)) * a.q_stride +
                       (kv_head * group + (in ? row - token * group : 0)) * kDim + 2 * t4;
 #pragma unroll
       for (int k = 0; k < kDim / 16; ++k) {
-        q[k][e] = in ? __ldg(reinterpret_cast<const uint32_t*>(from + 16 * k)) : 0u;
-        q[k][2 + e] = in ? __ldg(reinterpret_cast<const uint32_t*>(from + 16 * k + 8)) : 0u;
+        q[k][e] = in ? __ldcg(reinterpret_cast<const uint32_t*>(from + 16 * k)) : 0u;
+        q[k][2 + e] = in ? __ldcg(reinterpret_cast<const uint32_t*>(from + 16 * k + 8)) : 0u;
       }
     }
     float o[kDim / 8][4];
@@ -486,8 +492,7 @@ __global__ void __launch_bounds__(FewShared<kDim>::kThreads, FewShared<kDim>::kC
         }
         if (poisoned) {
           const int position = tile.first_position + token;
-          const int low = max((tile.block_begin + block) * kBlock,
-                              a.sliding_window > 0 ? position - a.sliding_window + 1 : 0);
+          const int low = max((tile.block_begin + block) * kBlock, first_visible(position, a.sliding_window));
           const int high = min((tile.block_begin + block + count) * kBlock - 1, position);
           sum.x += nonfinite_sum<T, kDim>(a, s, kv_head, low, high, column);
           sum.y += nonfinite_sum<T, kDim>(a, s, kv_head, low, high, column + 1);
@@ -643,8 +648,10 @@ cudaError_t launch_few(const PagedAttentionArgs& a, int most, cudaStream_t strea
 // where a 256-row tile of the chunk kernel would be nearly empty; the others to the chunk kernel. Only
 // what the bound on the new tokens allows for is launched, and a batch of one sequence with a larger
 // bound takes the chunk kernel alone: the launches it would save cost more than a short chunk there.
-// FORM_TIMES
-constexpr int kFewRows = 32;
+// Both forms at 7 heads a KV head, this one first: 6 tokens (42 rows), one sequence over 4K keys 18.3 and
+// 34.0 us, 16 sequences over 512 keys 20.1 and 25.5, over 4K keys 59.9 and 55.6; 9 tokens (63 rows), 16
+// sequences over 4K keys 74.1 and 58.6.
+constexpr int kFewRows = 48;
 
 struct FormChoice {
   int few_tokens = 0;  // new tokens up to which a sequence takes the few-row form; 0: not launched

@@ -9,11 +9,13 @@
 //   warp 8          TMA: Q of both halves, K and V blocks into a ring of four stages
 //   warp 9          tcgen05.mma of both halves
 // TMEM: S0 | S1 | O0 | O1, 128 columns each; P (16-bit) overwrites its S. Per half and block:
-//   S = Q K^T;  softmax warps read S, write P in two halves of 64 keys;  O += P V starts with the first
-//   while the second is being computed;  the next S follows behind it.
+//   S = Q K^T;  softmax warps read S and write P, 96 keys, then 32;  O += P V starts with the first
+//   while the others are being computed;  the next S follows behind it.
 // While one half's products run, the other half's softmax does.
-// Bounds: 4 x 128^3 x 2 FLOP a block and half pair against 2 x 128 x 128 exponentials at 16 a clock and
-// SM: the tensor pipe and the exponentials each take 2048 clocks a block.
+// Bounds: the products of a block take the tensor pipe 2048 clocks, its 2 x 128 x 128 exponentials the
+// SFU as many (16 a clock and SM). A half's chain, scores - softmax - P V - next scores, is about 3400
+// clocks long, of which the pipe works 2048; two 4K chunks over up to 8K keys (825 GFLOP) take 780 to
+// 860 us, 0.59 to 0.64 of the measured burst, at clocks that fall to 1.55 GHz under the power limit.
 //
 // Work: the (tile, KV head, key block) units form one line that is cut into equal parts, one a CTA
 // (paged_plan.cuh); tiles that a part does not hold whole leave fp32 partial sums, which the joining
@@ -344,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------------------------------- MMA
     // The halves' products are issued in turn, [O += P V, next S] of half 0, then of half 1, which keeps
     // the halves half a block apart: with a warp for each half they fell into step, their exponentials
-    // sharing the SFU and their products the tensor pipe (985 against 735 us for two 4K chunks).
+    // sharing the SFU and their products the tensor pipe (985 against 880 us for two 4K chunks).
     const uint32_t elected = elect_one();
     uint32_t turn = 0;  // blocks so far
     uint32_t segment = 0;

@@ -422,6 +422,10 @@ ATTENTION_CASES = {
     "fewer cached than new": ([(10, 4), (50, 3), (3, 0), (200, 130), (1, 0), (5, 5)], 8, 2, 128, 16, 0, "fp16"),
     "fewer cached than new window": ([(10, 4), (50, 3), (3, 0), (200, 130), (1, 0)], 28, 4, 64, 16, 7, "bf16"),
     "single none cached": ([(1, 0), (1, 5), (1, 0)], 28, 4, 128, 16, 0, "fp16"),
+    "forty rows": ([(6, 100), (5, 700), (1, 64), (6, 6), (3, 65)], 28, 4, 128, 16, 0, "fp16"),
+    "forty rows window": ([(6, 100), (5, 700), (1, 64), (6, 6), (3, 65)], 28, 4, 64, 32, 50, "bf16"),
+    "largest window": ([(10, 4), (50, 3), (3, 0), (200, 130), (1, 0), (5, 5)], 8, 2, 128, 16, 2**31 - 1, "fp16"),
+    "largest window few": ([(4, 1), (3, 0), (4, 200), (1, 0), (2, 2)], 8, 2, 64, 16, 2**31 - 1, "bf16"),
     "long": ([(1, 20_000), (2, 9000)], 28, 4, 128, 64, 0, "fp16"),
     "long chunk": ([(100, 9000)], 14, 2, 128, 64, 0, "bf16"),
     "long chunk window": ([(700, 9000)], 14, 2, 128, 16, 3000, "bf16"),
@@ -464,6 +468,22 @@ def test_paged_attention_rising_scores(cuda, chunk):
     q.view(-1, heads, dim)[..., 0] = 64.0
     out, lse = torch.empty_like(q), torch.empty(paged.tokens, heads, device=cuda)
     paged.attention(q, heads, out, lse)
+    check_attention(paged, q, out, lse, heads)
+
+
+@pytest.mark.parametrize("chunk", [1, 5, 60])
+def test_paged_attention_shared_prefix_pages(cuda, chunk):
+    """Sequences whose first pages are the same ones: the instruction all prompts begin with."""
+    import torch
+    heads, kv_heads, dim, page, prefix = 14, 2, 128, 16, 96
+    paged = Paged(cuda, [(chunk, prefix + 70), (chunk, prefix + chunk), (chunk, prefix + 300)], kv_heads, dim, page, "fp16", seed=4)
+    for s in (1, 2):
+        paged.tables[s][:prefix // page] = paged.tables[0][:prefix // page]
+        paged.table[s, :prefix // page] = paged.table[0, :prefix // page]
+    q = torch.randn(paged.tokens, heads * dim, generator=paged.generator, device=cuda).half()
+    out, lse = torch.empty_like(q), torch.empty(paged.tokens, heads, device=cuda)
+    paged.attention(q, heads, out, lse)
+    assert int(paged.status) == 0
     check_attention(paged, q, out, lse, heads)
 
 
