@@ -179,6 +179,7 @@ int ar_rotary_positions(const void* x, int64_t x_token_stride, int64_t x_head_st
     const char* who = "rotary_positions";
     require(dtype == AR_DTYPE_F16 || dtype == AR_DTYPE_BF16, who, "dtype must be fp16 or bf16");
     require(token_count >= 0 && heads >= 0 && table_positions >= 0, who, "counts must not be negative");
+    require(heads <= 65536, who, "heads must be at most 65536");
     require(head_dim >= 2 && head_dim <= 1024, who, "head_dim must be 2..1024");
     require(rotary_dim >= 2 && rotary_dim <= head_dim && rotary_dim % 2 == 0, who,
             "rotary_dim must be even, 2..head_dim");
@@ -295,6 +296,9 @@ int ar_paged_attention(const ar_paged_cache* cache, const ar_paged_batch* batch,
     require(q_stride >= width && q_stride % 8 == 0 && out_stride >= width && out_stride % 8 == 0, who,
             "q_stride and out_stride must be multiples of 8 and hold the query heads");
     require(std::isfinite(scale) && scale >= 0.0f, who, "scale must be finite and not negative (0: 1/sqrt(head_dim))");
+    const double chosen = scale != 0.0f ? scale : 1.0 / std::sqrt(static_cast<double>(args.cache.head_dim));
+    args.scale_log2 = static_cast<float>(chosen * 1.4426950408889634074);
+    require(std::isnormal(args.scale_log2), who, "scale times log2(e) must be a normal fp32 number");
     require(sliding_window >= 0, who, "sliding_window must not be negative");
     if (args.batch.tokens == 0 || args.batch.sequences == 0) return AR_OK;
     require(q != nullptr && out != nullptr && aligned16(q) && aligned16(out), who,
@@ -307,8 +311,6 @@ int ar_paged_attention(const ar_paged_cache* cache, const ar_paged_batch* batch,
     args.q = q;
     args.q_stride = q_stride;
     args.query_heads = query_heads;
-    const double chosen = scale != 0.0f ? scale : 1.0 / std::sqrt(static_cast<double>(args.cache.head_dim));
-    args.scale_log2 = static_cast<float>(chosen * 1.4426950408889634074);
     args.sliding_window = sliding_window;
     args.out = out;
     args.out_stride = out_stride;

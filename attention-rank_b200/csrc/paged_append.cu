@@ -18,7 +18,7 @@ constexpr int kThreads = 256;
 template <typename T, bool kInterleaved, bool kBias, int kHeads, int kTokens>
 __global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppendArgs a, int first_head, int units,
                                                                 int rotated_units, int groups) {
-  static_assert(kTokens <= kThreads / 32, "one warp finds each row's place");
+  static_assert(kTokens < kThreads / 32, "one warp finds each row's place, another checks the batch");
   __shared__ int position_of[kTokens];
   __shared__ int64_t slot_of[kTokens];
   const int begin = blockIdx.x * kTokens;
@@ -53,6 +53,10 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppen
     if ((threadIdx.x & 31) == 0) {
       position_of[warp] = position;
       slot_of[warp] = slot;
+    }
+  } else if (warp == kTokens) {  // sequences out of range are reported even where no row leads to them
+    for (int64_t s = blockIdx.x * 32 + (threadIdx.x & 31); s < a.batch.sequences; s += gridDim.x * 32) {
+      paged_sequence(a.batch, static_cast<int>(s), a.status);
     }
   }
   __syncthreads();

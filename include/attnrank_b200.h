@@ -354,8 +354,8 @@ int ar_rope_table_scaled(const ar_rope_scaling* scaling, int positions, float* c
  * rotates back, which is also the gradient with respect to x. The other values are copied. out has
  * its own strides; out == x with x's strides works in place, any other overlap is undefined. A
  * position outside [0, table_positions) sets *device_status (nullable) to 2 and leaves its token's
- * rows of out as they were. rotary_dim is even, 2..head_dim, head_dim <= 1024, positions int32
- * [token_count], tables fp32 [table_positions, rotary_dim / 2]. Arithmetic in fp32, one rounding. */
+ * rows of out as they were. rotary_dim is even, 2..head_dim, head_dim <= 1024, heads <= 65536,
+ * positions int32 [token_count], tables fp32 [table_positions, rotary_dim / 2]. Arithmetic in fp32, one rounding. */
 int ar_rotary_positions(const void* x, int64_t x_token_stride, int64_t x_head_stride, void* out,
                         int64_t out_token_stride, int64_t out_head_stride, const int32_t* positions, int token_count,
                         int heads, int head_dim, int rotary_dim, int interleaved, int inverse, const float* cos_table,
@@ -423,7 +423,8 @@ int64_t ar_paged_attention_workspace(const ar_paged_cache* cache, const ar_paged
  * positions a row does not see, and slots past kv_lengths[s], do not touch it, whatever they hold.
  * q: 16-bit, row stride q_stride elements, heads of a row contiguous; out: 16-bit, row stride
  * out_stride, not overlapping q; both 16-byte aligned with strides multiples of 8. lse (nullable):
- * fp32 [token_count][query_heads]. scale 0 means 1/sqrt(head_dim). query_heads / kv_heads <= 128.
+ * fp32 [token_count][query_heads]. scale 0 means 1/sqrt(head_dim); scale log2(e) is a normal fp32
+ * number. query_heads / kv_heads <= 128, and no sequence may have more than 2^24 new tokens.
  * Scores, softmax statistics and sums are fp32; the probabilities are rounded to the 16-bit type for
  * the product with v. Rows no sequence owns are left as they were. The same call on the same data
  * gives the same bits. workspace: 16-byte aligned, its contents mean nothing between calls; calls

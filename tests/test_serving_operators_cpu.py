@@ -107,6 +107,7 @@ def test_bad_scalings_are_refused_by_both_entry_points(name):
 TABLE = dict(positions=16, cos=ADDRESS, sin=ADDRESS)
 BAD_TABLES = {
     "negative positions": (dict(positions=-1), "positions"),
+    "too many positions": (dict(positions=(1 << 30) + 1), "positions"),
     "null cos": (dict(cos=None), "16-byte aligned"),
     "unaligned sin": (dict(sin=ADDRESS + 4), "16-byte aligned"),
 }
@@ -127,6 +128,7 @@ BAD_ROTARY = {
     "fp32": (dict(dtype=0), "dtype"),
     "negative tokens": (dict(tokens=-1), "counts"),
     "negative heads": (dict(heads=-1), "counts"),
+    "too many heads": (dict(heads=65537), "65536"),
     "negative table": (dict(table=-1), "counts"),
     "head_dim": (dict(head_dim=1025), "head_dim"),
     "odd rotary": (dict(rotary=63), "even"),
@@ -255,6 +257,9 @@ BAD_ATTENTIONS = {
     "short out": (dict(out_stride=27 * 128), "out_stride"),
     "negative scale": (dict(scale=-0.5), "scale"),
     "nan scale": (dict(scale=math.nan), "scale"),
+    "scale beyond fp32 in log2": (dict(scale=3e38), "normal"),
+    "subnormal scale": (dict(scale=1e-45), "normal"),
+    "2^24 + 1 new tokens": (dict(most=(1 << 24) + 1, tokens=(1 << 24) + 1), "2^24"),
     "negative window": (dict(window=-1), "sliding_window"),
     "null q": (dict(q=None), "q and out"),
     "unaligned out": (dict(out=ADDRESS + 8), "q and out"),

@@ -612,6 +612,30 @@ def test_bad_batches_are_reported_and_left_out(cuda, name, heads):
         assert torch.equal(paged.k[ids].nan_to_num(), k[ids].nan_to_num()) and torch.equal(paged.v[ids].nan_to_num(), v[ids].nan_to_num())
 
 
+@pytest.mark.parametrize("new", [1, 300])
+def test_idle_sequences_out_of_range_are_reported(cuda, new):
+    """Sequence 1 has no new tokens and a negative length: no row leads to it, both operators report it."""
+    import torch
+    native = _lib()
+    paged = Paged(cuda, [(new, 320), (0, 25), (1, 30)], 2, 64, 16, "fp16")
+    paged.lengths[1] = -1
+    q = torch.randn(paged.tokens, 4 * 64, device=cuda).half()
+    out, lse = torch.full_like(q, SENTINEL), torch.full((paged.tokens, 4), SENTINEL, device=cuda)
+    paged.attention(q, 4, out, lse)
+    torch.cuda.synchronize()
+    assert int(paged.status) == 4
+    check_attention(paged, q, out, lse, 4, rows_of=[0, 2])
+    paged.status.zero_()
+    qkv = torch.randn(paged.tokens, 8 * 64, device=cuda).half()
+    native.check(native.lib.ar_paged_append(ctypes.byref(paged.cache), ctypes.byref(paged.batch), qkv.data_ptr(), 8 * 64, None,
+                                            4, None, 0, None, None, 0, 0, 0, paged.status.data_ptr(), _stream()))
+    torch.cuda.synchronize()
+    assert int(paged.status) == 4
+    row = qkv[-1].view(8, 64)
+    page = int(paged.tables[2][29 // 16])
+    assert torch.equal(paged.k[page, :, 29 % 16], row[4:6]) and torch.equal(paged.v[page, :, 29 % 16], row[6:])
+
+
 @pytest.mark.parametrize("new", [1, 40])
 @pytest.mark.parametrize("page_id", [-1, 10**6, 2**31 - 1, -2**31])
 def test_page_ids_outside_the_pool_are_reported(cuda, page_id, new):
