@@ -179,6 +179,8 @@ SIGNATURES: dict[str, list] = {
     "ar_paged_attention_workspace": [ctypes.POINTER(PagedCacheStruct), ctypes.POINTER(PagedBatchStruct), _I],
     "ar_paged_attention": [ctypes.POINTER(PagedCacheStruct), ctypes.POINTER(PagedBatchStruct), _P, _I64, _I, _F, _I, _P,
                            _I64, _P, _P, _I64, _P, _P],
+    "ar_paged_attention_wait_selftest": [ctypes.POINTER(PagedCacheStruct), ctypes.POINTER(PagedBatchStruct), _P, _I64, _I, _I,
+                                         _P, _I64, _P, _P, _I64, ctypes.c_uint32, _P, _P],
     "ar_bounded_wait_selftest": [_I, ctypes.c_uint32, _P],
     "ar_profile_from_accumulated": [_P, _I, _I64, _P, _P],
     "ar_position_order": [_P, _I, _P],

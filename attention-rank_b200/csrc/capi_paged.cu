@@ -135,6 +135,47 @@ void check_query_heads(const char* who, int query_heads, const arb::PagedCache& 
           "query_heads must be a positive multiple of kv_heads, at most 128 times it");
 }
 
+int attention_call(const char* who, const ar_paged_cache* cache, const ar_paged_batch* batch, const void* q,
+                   int64_t q_stride, int query_heads, float scale, int sliding_window, void* out, int64_t out_stride,
+                   float* lse, void* workspace, int64_t workspace_bytes, int* device_status, void* stream,
+                   uint32_t self_test_blocks) {
+  arb::PagedAttentionArgs args;
+  args.cache = checked_cache(who, cache);
+  args.batch = checked_batch(who, batch, args.cache);
+  check_query_heads(who, query_heads, args.cache);
+  require(args.batch.max_query <= 1 << 24, who, "max_query_tokens must be at most 2^24");
+  const int64_t width = static_cast<int64_t>(query_heads) * args.cache.head_dim;
+  require(q_stride >= width && q_stride % 8 == 0 && out_stride >= width && out_stride % 8 == 0, who,
+          "q_stride and out_stride must be multiples of 8 and hold the query heads");
+  require(std::isfinite(scale) && scale >= 0.0f, who, "scale must be finite and not negative (0: 1/sqrt(head_dim))");
+  const double chosen = scale != 0.0f ? scale : 1.0 / std::sqrt(static_cast<double>(args.cache.head_dim));
+  args.scale_log2 = static_cast<float>(chosen * 1.4426950408889634074);
+  require(std::isnormal(args.scale_log2), who, "scale times log2(e) must be a normal fp32 number");
+  require(sliding_window >= 0, who, "sliding_window must not be negative");
+  if (args.batch.tokens == 0 || args.batch.sequences == 0) return AR_OK;
+  require(q != nullptr && out != nullptr && aligned16(q) && aligned16(out), who,
+          "q and out must be 16-byte aligned device arrays");
+  require(q != out, who, "out must not overlap q");
+  const int64_t needed = arb::paged_attention_workspace(args.cache, args.batch, query_heads);
+  if (needed > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < needed)) {
+    throw arb::Error(std::string(who) + ": needs a 16-byte aligned workspace of " + std::to_string(needed) + " bytes");
+  }
+  args.q = q;
+  args.q_stride = q_stride;
+  args.query_heads = query_heads;
+  args.sliding_window = sliding_window;
+  args.out = out;
+  args.out_stride = out_stride;
+  args.lse = lse;
+  args.workspace = workspace;
+  args.status = device_status;
+  args.self_test_blocks = self_test_blocks;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  ArrayDevice device(cache->k_pages);
+  arb::check_cuda(arb::launch_paged_attention(args, s), who);
+  return AR_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -286,41 +327,18 @@ int ar_paged_attention(const ar_paged_cache* cache, const ar_paged_batch* batch,
                        int query_heads, float scale, int sliding_window, void* out, int64_t out_stride, float* lse,
                        void* workspace, int64_t workspace_bytes, int* device_status, void* stream) {
   return arb::guarded_call([&] {
-    const char* who = "paged_attention";
-    arb::PagedAttentionArgs args;
-    args.cache = checked_cache(who, cache);
-    args.batch = checked_batch(who, batch, args.cache);
-    check_query_heads(who, query_heads, args.cache);
-    require(args.batch.max_query <= 1 << 24, who, "max_query_tokens must be at most 2^24");
-    const int64_t width = static_cast<int64_t>(query_heads) * args.cache.head_dim;
-    require(q_stride >= width && q_stride % 8 == 0 && out_stride >= width && out_stride % 8 == 0, who,
-            "q_stride and out_stride must be multiples of 8 and hold the query heads");
-    require(std::isfinite(scale) && scale >= 0.0f, who, "scale must be finite and not negative (0: 1/sqrt(head_dim))");
-    const double chosen = scale != 0.0f ? scale : 1.0 / std::sqrt(static_cast<double>(args.cache.head_dim));
-    args.scale_log2 = static_cast<float>(chosen * 1.4426950408889634074);
-    require(std::isnormal(args.scale_log2), who, "scale times log2(e) must be a normal fp32 number");
-    require(sliding_window >= 0, who, "sliding_window must not be negative");
-    if (args.batch.tokens == 0 || args.batch.sequences == 0) return AR_OK;
-    require(q != nullptr && out != nullptr && aligned16(q) && aligned16(out), who,
-            "q and out must be 16-byte aligned device arrays");
-    require(q != out, who, "out must not overlap q");
-    const int64_t needed = arb::paged_attention_workspace(args.cache, args.batch, query_heads);
-    if (needed > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < needed)) {
-      throw arb::Error(std::string(who) + ": needs a 16-byte aligned workspace of " + std::to_string(needed) + " bytes");
-    }
-    args.q = q;
-    args.q_stride = q_stride;
-    args.query_heads = query_heads;
-    args.sliding_window = sliding_window;
-    args.out = out;
-    args.out_stride = out_stride;
-    args.lse = lse;
-    args.workspace = workspace;
-    args.status = device_status;
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    ArrayDevice device(cache->k_pages);
-    arb::check_cuda(arb::launch_paged_attention(args, s), who);
-    return AR_OK;
+    return attention_call("paged_attention", cache, batch, q, q_stride, query_heads, scale, sliding_window, out, out_stride,
+                          lse, workspace, workspace_bytes, device_status, stream, ~0u);
+  });
+}
+
+int ar_paged_attention_wait_selftest(const ar_paged_cache* cache, const ar_paged_batch* batch, const void* q,
+                                     int64_t q_stride, int query_heads, int sliding_window, void* out, int64_t out_stride,
+                                     float* lse, void* workspace, int64_t workspace_bytes, uint32_t blocks,
+                                     int* device_status, void* stream) {
+  return arb::guarded_call([&] {
+    return attention_call("paged_attention_wait_selftest", cache, batch, q, q_stride, query_heads, 0.0f, sliding_window, out,
+                          out_stride, lse, workspace, workspace_bytes, device_status, stream, blocks);
   });
 }
 

@@ -97,6 +97,7 @@ struct PagedAttentionArgs {
   float* lse = nullptr;
   void* workspace = nullptr;
   int* status = nullptr;
+  uint32_t self_test_blocks = ~0u;  // key blocks of its part that a CTA loads; the waits for more run out
 };
 int64_t paged_attention_workspace(const PagedCache& cache, const PagedBatch& batch, int query_heads);
 cudaError_t launch_paged_attention(const PagedAttentionArgs& args, cudaStream_t stream);

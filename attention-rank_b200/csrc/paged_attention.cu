@@ -237,7 +237,10 @@ __global__ void __launch_bounds__(FewShared<kDim>::kThreads, FewShared<kDim>::kC
         const int following = i + 1 < count ? page_at(block + i + 1) : -1;  // its latency hides behind the wait
         const int stage = turn % kStages;
         const uint32_t round = turn / kStages;
-        if (round > 0 && !mbar_wait(smem_u32(&sh.empty[stage]), (round - 1) & 1, &sh.abort)) {
+        // the whole warp goes on or stops; a warp that gave up arrives no more, so a stage that is free
+        // has landed as well
+        const bool free = round == 0 || mbar_wait(smem_u32(&sh.empty[stage]), (round - 1) & 1, &sh.abort);
+        if (!__all_sync(0xffffffffu, free && turn < a.self_test_blocks)) {
           ok = false;
           break;
         }
@@ -258,19 +261,19 @@ __global__ void __launch_bounds__(FewShared<kDim>::kThreads, FewShared<kDim>::kC
       left -= count;
       if (left > 0) next_tile();
     }
-    if (!ok) {  // a consumer gave up: the loads in flight land before the shared memory is released
-      if (lane == 0) {
-        report_status(a.status, kStatusWaitTimeout);
-        sh.abort = 1;
-      }
-      for (uint32_t t = turn > kStages ? turn - kStages : 0; t < turn; ++t) {
-        mbar_wait(smem_u32(&sh.full[t % kStages]), (t / kStages) & 1, nullptr);
-      }
+    if (!ok && turn < a.self_test_blocks && lane == 0) {
+      report_status(a.status, kStatusWaitTimeout);
+      sh.abort = 1;
+    }
+    // the loads in flight land before the shared memory is released, even if no consumer waits for them
+    for (uint32_t t = turn > kStages ? turn - kStages : 0; t < turn; ++t) {
+      mbar_wait(smem_u32(&sh.full[t % kStages]), (t / kStages) & 1, nullptr);
     }
     return;
   }
 
   // ------------------------------------------------------------------------------------ consumers
+  constexpr int kSegmentBarriers = 1 + 2 * (kDim / 32);  // of a segment, in the join of the warps' sums
   const int group = a.query_heads / a.cache.kv_heads;
   const int quarter = warp;  // the warp's 16 keys of a block
   const int g = lane >> 2;
@@ -293,7 +296,7 @@ __global__ void __launch_bounds__(FewShared<kDim>::kThreads, FewShared<kDim>::kC
   };
   bool ok = true;
   int segment = 0;
-  while (ok && left > 0) {
+  while (left > 0) {
     const int count = static_cast<int>(min(left, static_cast<int64_t>(tile.blocks - block)));
     const int rows = seq.q_len * group;
     // Q as MMA operands: the lane holds rows g and g + 8 of its group's 16
@@ -518,9 +521,17 @@ __global__ void __launch_bounds__(FewShared<kDim>::kThreads, FewShared<kDim>::kC
     left -= count;
     if (left > 0) next_tile();
   }
-  if (!ok && lane == 0) {
+  if (ok) return;
+  // A wait gave up: no later one lasts, but the other warps may have got through this one and stand at the
+  // barriers of this segment or the next ones, so this warp meets them there.
+  if (lane == 0) {
     report_status(a.status, kStatusWaitTimeout);
     sh.abort = 1;
+  }
+  while (left > 0) {
+    for (int i = 0; i < kSegmentBarriers; ++i) consumer_barrier();
+    left -= min(left, static_cast<int64_t>(tile.blocks - block));
+    if (left > 0) next_tile();
   }
 }
 

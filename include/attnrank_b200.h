@@ -428,10 +428,21 @@ int64_t ar_paged_attention_workspace(const ar_paged_cache* cache, const ar_paged
  * Scores, softmax statistics and sums are fp32; the probabilities are rounded to the 16-bit type for
  * the product with v. Rows no sequence owns are left as they were. The same call on the same data
  * gives the same bits. workspace: 16-byte aligned, its contents mean nothing between calls; calls
- * whose work may overlap on the GPU (two streams, two captured graphs) each need their own. */
+ * whose work may overlap on the GPU (two streams, two captured graphs) each need their own. Every wait
+ * inside the kernels is bounded: one that runs out (0.5 s, a stalled device) sets *device_status to 3
+ * and leaves rows of out and lse unspecified; pass a status word to learn of it. */
 int ar_paged_attention(const ar_paged_cache* cache, const ar_paged_batch* batch, const void* q, int64_t q_stride,
                        int query_heads, float scale, int sliding_window, void* out, int64_t out_stride, float* lse,
                        void* workspace, int64_t workspace_bytes, int* device_status, void* stream);
+
+/* Self-test of that call's bounded waits: the same work with scale 0, but a CTA loads only the first
+ * `blocks` key blocks of its share, so that the wait for the next one runs out. Where a share has more
+ * blocks than that, *device_status becomes 3 after about 0.5 s and rows of out and lse are unspecified;
+ * nothing else is touched and the device stays usable. */
+int ar_paged_attention_wait_selftest(const ar_paged_cache* cache, const ar_paged_batch* batch, const void* q,
+                                     int64_t q_stride, int query_heads, int sliding_window, void* out, int64_t out_stride,
+                                     float* lse, void* workspace, int64_t workspace_bytes, uint32_t blocks,
+                                     int* device_status, void* stream);
 
 /* Self-test of the library's bounded device waits. No counterpart in the reference: its kernels
  * never wait on one another. `ctas` CTAs (1..1024) wait on the grid barrier of the persistent
