@@ -140,18 +140,36 @@ __device__ __forceinline__ uint32_t clean_pair(uint32_t pair, int key, int first
   return (in0 && !bad0 ? pair & 0xffffu : 0u) | (in1 && !bad1 ? pair & 0xffff0000u : 0u);
 }
 
-// Sum of the values of column `column` that are not finite, over the keys [first, last] of sequence s.
+// Does every row of the sequence see every key of the block that begins at key0?
+__device__ __forceinline__ bool whole_block(const PagedSequence& seq, const FewTile& t, int window, int key0) {
+  return key0 + kBlock - 1 <= t.first_position && (window == 0 || key0 >= seq.kv_len - window);
+}
+
+// Sums of what clean_pair cleared of columns [column, column + 4) at the keys that the row at `position`
+// sees: the values that are not finite, in those of the blocks [begin, end) that not every row sees whole.
+// That is a few blocks at either end of what the tile sees, however long the cache is, so that no wait
+// for this warp runs out meanwhile.
 template <typename T, int kDim>
-__device__ float nonfinite_sum(const PagedAttentionArgs& a, int s, int kv_head, int first, int last, int column) {
-  float sum = 0.0f;
-  for (int key = first; key <= last; ++key) {
-    const int page = paged_page(a.cache, a.batch, s, key >> a.cache.page_shift, a.status);
-    const int64_t row = ((static_cast<int64_t>(page) * a.cache.kv_heads + kv_head) << a.cache.page_shift) +
-                        (key & ((1 << a.cache.page_shift) - 1));
-    const float v = static_cast<float>(static_cast<const T*>(a.cache.v_pages)[row * kDim + column]);
-    if (!isfinite(v)) sum += v;
+__device__ __forceinline__ float4 nonfinite_sums(const PagedAttentionArgs& a, int s, const PagedSequence& seq,
+                                                 const FewTile& t, int begin, int end, int kv_head, int position, int column) {
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int block = t.block_begin + begin; block < t.block_begin + end; ++block) {
+    if (whole_block(seq, t, a.sliding_window, block * kBlock)) continue;
+    const int first = max(block * kBlock, first_visible(position, a.sliding_window));
+    const int last = min(block * kBlock + kBlock - 1, position);
+    for (int key = first; key <= last; ++key) {
+      const int page = paged_page(a.cache, a.batch, s, key >> a.cache.page_shift, a.status);
+      const int64_t row = ((static_cast<int64_t>(page) * a.cache.kv_heads + kv_head) << a.cache.page_shift) +
+                          (key & ((1 << a.cache.page_shift) - 1));
+      const T* v = static_cast<const T*>(a.cache.v_pages) + row * kDim + column;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float value = static_cast<float>(v[i]);
+        if (!isfinite(value)) sum[i] += value;
+      }
+    }
   }
-  return sum;
+  return make_float4(sum[0], sum[1], sum[2], sum[3]);
 }
 
 template <typename T, int kDim>
@@ -349,8 +367,7 @@ __global__ void __launch_bounds__(FewShared<kDim>::kThreads, FewShared<kDim>::kC
       const int key0 = (tile.block_begin + block + i) * kBlock;
       const int key = key0 + quarter * 16 + 2 * t4;  // of x[0][0]
       // does every row see every key of the block?
-      const bool whole = key0 + kBlock - 1 <= tile.first_position &&
-                         (a.sliding_window == 0 || key0 >= seq.kv_len - a.sliding_window);
+      const bool whole = whole_block(seq, tile, a.sliding_window, key0);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
 #pragma unroll
@@ -494,13 +511,12 @@ __global__ void __launch_bounds__(FewShared<kDim>::kThreads, FewShared<kDim>::kC
           sum.w += part.w;
         }
         if (poisoned) {
-          const int position = tile.first_position + token;
-          const int low = max((tile.block_begin + block) * kBlock, first_visible(position, a.sliding_window));
-          const int high = min((tile.block_begin + block + count) * kBlock - 1, position);
-          sum.x += nonfinite_sum<T, kDim>(a, s, kv_head, low, high, column);
-          sum.y += nonfinite_sum<T, kDim>(a, s, kv_head, low, high, column + 1);
-          sum.z += nonfinite_sum<T, kDim>(a, s, kv_head, low, high, column + 2);
-          sum.w += nonfinite_sum<T, kDim>(a, s, kv_head, low, high, column + 3);
+          const float4 more = nonfinite_sums<T, kDim>(a, s, seq, tile, block, block + count, kv_head,
+                                                      tile.first_position + token, column);
+          sum.x += more.x;
+          sum.y += more.y;
+          sum.z += more.z;
+          sum.w += more.w;
         }
         if (complete) {
           T* to = static_cast<T*>(a.out) + (seq.q_begin + token) * a.out_stride + head * kDim + column;

@@ -158,25 +158,40 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t pair) {
   return pair & ~((nonfinite_pair<T>(pair) >> 15) * 0xffffu);
 }
 
-// Adds to a row, written by this thread, the values of V that are not finite at the keys [first, last]
-// it sees. `out` is the row in the 16-bit result, or NULL and `sums` its place in the partial sums.
+// Adds to a row, written by this thread, what was cleared of the segment's V at the keys [row_first,
+// row_last] it sees: the values that are not finite, in the blocks that not every row of the tile sees
+// whole. That is a few blocks at either end of what the tile sees, however long the cache is, so that no
+// wait for this warp runs out meanwhile. `out` is the row in the 16-bit result, or NULL and `sums` its
+// place in the partial sums.
 template <typename T, int kDim>
-__device__ __noinline__ void add_nonfinite(const PagedAttentionArgs& a, int s, int kv_head, int first, int last, T* out,
+__device__ __noinline__ void add_nonfinite(const PagedAttentionArgs& a, const Walk w, int row_first, int row_last, T* out,
                                            float* sums) {
-  for (int column = 0; column < kDim; ++column) {
-    float more = 0.0f;
-    for (int key = first; key <= last; ++key) {
-      const int page = paged_page(a.cache, a.batch, s, key >> a.cache.page_shift, a.status);
-      const int64_t row = ((static_cast<int64_t>(page) * a.cache.kv_heads + kv_head) << a.cache.page_shift) +
+  for (int b = w.block; b < w.block + w.count; ++b) {
+    if (w.whole(b, a.sliding_window)) continue;
+    const int key0 = (w.tile.block_begin + b) * kChunkBlock;
+    for (int key = max(key0, row_first); key <= min(key0 + kChunkBlock - 1, row_last); ++key) {
+      const int page = paged_page(a.cache, a.batch, w.s, key >> a.cache.page_shift, a.status);
+      const int64_t row = ((static_cast<int64_t>(page) * a.cache.kv_heads + w.kv_head) << a.cache.page_shift) +
                           (key & ((1 << a.cache.page_shift) - 1));
-      const float v = static_cast<float>(static_cast<const T*>(a.cache.v_pages)[row * kDim + column]);
-      if (!isfinite(v)) more += v;
-    }
-    if (more == 0.0f) continue;  // all of them finite
-    if (out != nullptr) {
-      out[column] = static_cast<T>(static_cast<float>(out[column]) + more);
-    } else {
-      sums[(column >> 2) * (2 * kRows * 4) + (column & 3)] += more;
+      const uint4* v = reinterpret_cast<const uint4*>(static_cast<const T*>(a.cache.v_pages) + row * kDim);
+#pragma unroll 4
+      for (int i = 0; i < kDim / 8; ++i) {
+        const uint4 raw = v[i];
+        if ((nonfinite_pair<T>(raw.x) | nonfinite_pair<T>(raw.y) | nonfinite_pair<T>(raw.z) | nonfinite_pair<T>(raw.w)) == 0) {
+          continue;
+        }
+        float value[8];
+        unpack8<T>(raw, value);
+        for (int j = 0; j < 8; ++j) {
+          const int column = 8 * i + j;
+          if (isfinite(value[j])) continue;
+          if (out != nullptr) {
+            out[column] = static_cast<T>(static_cast<float>(out[column]) + value[j]);
+          } else {
+            sums[(column >> 2) * (2 * kRows * 4) + (column & 3)] += value[j];
+          }
+        }
+      }
     }
   }
 }
@@ -665,8 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       mbar_arrive_if(elected, smem_u32(&ctl.o_free[half]));
       if (row_in && poisoned) {
-        add_nonfinite<T, kDim>(a, w.s, w.kv_head, max(row_first, (w.tile.block_begin + w.block) * kChunkBlock),
-                               min(row_last, (w.tile.block_begin + end) * kChunkBlock - 1),
+        add_nonfinite<T, kDim>(a, w, row_first, row_last,
                                complete ? static_cast<T*>(a.out) + out_token * a.out_stride + head * kDim : nullptr,
                                partials.sums + (slot * (2 * kRows) * (kDim / 4) + half * kRows + row) * 4);
       }
