@@ -290,7 +290,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 8) {
     // ------------------------------------------------------------------------------------- TMA
+    // The whole warp goes on or stops. A barrier is armed again only after its last load has landed, whatever
+    // the MMA warp waited for: it runs on after a wait that gave up.
     bool ok = true;
+    auto freed = [&](uint64_t& empty, uint64_t& full, uint32_t phase) {
+      return __all_sync(0xffffffffu, mbar_wait_called(smem_u32(&empty), phase, &ctl.abort) &&
+                                         mbar_wait_called(smem_u32(&full), phase, &ctl.abort)) != 0;
+    };
     const int page_rows = min(1 << a.cache.page_shift, kChunkBlock);
     const int boxes = kChunkBlock / page_rows * kHalves;
     const int my_page = lane / kHalves;  // the lane's box: page and 64-wide half
@@ -298,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t item = 0;
     uint32_t segment = 0;
     do {
-      if (segment > 0 && !mbar_wait_called(smem_u32(&ctl.q_empty), (segment - 1) & 1, &ctl.abort)) {
+      if (segment > 0 && !freed(ctl.q_empty, ctl.q_full, (segment - 1) & 1)) {
         ok = false;
         break;
       }
@@ -330,7 +336,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv, ++item) {
           const uint32_t stage = stage_of(item);
-          if (item >= kStages && !mbar_wait_called(smem_u32(&ctl.empty[stage]), phase_of(item) ^ 1, &ctl.abort)) {
+          if ((item >= kStages && !freed(ctl.empty[stage], ctl.full[stage], phase_of(item) ^ 1)) ||
+              item >> 1 >= a.self_test_blocks) {
             ok = false;
             break;
           }
@@ -346,16 +353,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         page = following;
       }
     } while (ok && walk_next(w, c));
-    if (!ok) {
-      if (lane == 0) {
-        report_status(a.status, kStatusWaitTimeout);
-        ctl.abort = 1;
-      }
-      // the loads in flight land before the shared memory is released
-      if (segment > 0) mbar_wait_called(smem_u32(&ctl.q_full), (segment - 1) & 1, nullptr);
-      for (uint32_t i = item > kStages ? item - kStages : 0; i < item; ++i) {
-        mbar_wait_called(smem_u32(&ctl.full[stage_of(i)]), phase_of(i), nullptr);
-      }
+    if (!ok && item >> 1 < a.self_test_blocks && lane == 0) {
+      report_status(a.status, kStatusWaitTimeout);
+      ctl.abort = 1;
+    }
+    // the loads in flight land before the shared memory is released, even if the MMA warp no longer waits for them
+    if (segment > 0) mbar_wait_called(smem_u32(&ctl.q_full), (segment - 1) & 1, nullptr);
+    for (uint32_t i = item > kStages ? item - kStages : 0; i < item; ++i) {
+      mbar_wait_called(smem_u32(&ctl.full[stage_of(i)]), phase_of(i), nullptr);
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------------------------------- MMA

@@ -73,3 +73,18 @@ def test_few_row_waits_that_run_out(cuda, name, blocks):
 
 def test_few_row_waits_that_run_out_at_64_with_a_window(cuda):
     check_waits(cuda, FEW["singles"], 8, 8, 64, 64, 300, "bf16", [2, 2])
+
+
+CHUNKS = [(300, 4000), (512, 2500), (130, 130), (700, 1900), (64, 3000), (257, 300)]
+
+
+@pytest.mark.parametrize("blocks", [0, 1, 2, 3, 5])
+@pytest.mark.parametrize("heads,kv_heads,head_dim,page,window,name", [(28, 4, 128, 64, 0, "fp16"), (16, 16, 64, 16, 500, "bf16")])
+def test_chunk_waits_that_run_out(cuda, heads, kv_heads, head_dim, page, window, name, blocks):
+    """Part of a CTA's loads are under way, or none, when the MMA and softmax warps give up."""
+    check_waits(cuda, CHUNKS, heads, kv_heads, head_dim, page, window, name, [blocks])
+
+
+def test_both_forms_of_a_mixed_batch_run_out(cuda):
+    """The few-row kernel's waits run out and then the chunk kernel's, one after the other."""
+    check_waits(cuda, CHUNKS + FEW["singles"], 28, 4, 128, 16, 0, "bf16", [2])
