@@ -133,9 +133,10 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedBatch& b, int
   return {begin, end - begin, length};
 }
 
-// The sequence whose rows hold `token`, or -1; the whole warp calls it with the same token. Each
-// round probes 32 evenly spaced offsets, so 1024 sequences take two dependent loads.
-__device__ __forceinline__ int paged_sequence_of(const PagedBatch& b, int token) {
+// Where `token` lies among the offsets: the sequence whose rows hold it if they never decrease, else any
+// sequence or -1. The whole warp calls it with the same token. Each round probes 32 evenly spaced
+// offsets, so 1024 sequences take two dependent loads.
+__device__ __forceinline__ int paged_search(const PagedBatch& b, int token) {
   const int lane = threadIdx.x & 31;
   int low = 0;
   int count = b.sequences + 1;  // offsets not yet known to be above or not above `token`
@@ -148,6 +149,40 @@ __device__ __forceinline__ int paged_sequence_of(const PagedBatch& b, int token)
     count = max(0, min(step - 1, count - passed));
   }
   return low >= 1 && low <= b.sequences ? low - 1 : -1;
+}
+
+// The sequence whose rows hold `token` and that is in range (`seq`), or -1; the whole warp calls it with
+// the same token. Offsets that decrease somewhere mislead the search, so where it finds no such sequence,
+// though an offset lies behind the token, every one is looked at.
+__device__ __forceinline__ int paged_sequence_of(const PagedBatch& b, int token, int* status, PagedSequence& seq) {
+  const int lane = threadIdx.x & 31;
+  const int found = paged_search(b, token);
+  bool behind = false;
+  if (found >= 0) {
+    seq = paged_sequence(b, found, status);
+    if (token >= seq.q_begin && token - seq.q_begin < seq.q_len) return found;
+    behind = true;
+  } else {
+    // eight loads in flight: a row of padding waits for one round of them, not for each
+    for (int at = lane; at <= b.sequences; at += 256) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) behind |= __ldcg(b.q_offsets + min(at + 32 * i, b.sequences)) > token;
+    }
+  }
+  if (!__any_sync(0xffffffffu, behind)) return -1;  // rows behind the last sequence
+  for (int base = 0; base < b.sequences; base += 32) {
+    if (base + lane < b.sequences) seq = paged_sequence(b, base + lane, status);
+    const bool holds = base + lane < b.sequences && token >= seq.q_begin && token - seq.q_begin < seq.q_len;
+    const unsigned holders = __ballot_sync(0xffffffffu, holds);
+    if (holders != 0) {
+      const int owner = __ffs(holders) - 1;
+      seq.q_begin = __shfl_sync(0xffffffffu, seq.q_begin, owner);
+      seq.q_len = __shfl_sync(0xffffffffu, seq.q_len, owner);
+      seq.kv_len = __shfl_sync(0xffffffffu, seq.kv_len, owner);
+      return base + owner;
+    }
+  }
+  return -1;
 }
 
 // A page id of sequence s, clamped into the pool (an id outside it is reported).

@@ -27,26 +27,23 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppen
     const int token = begin + warp;
     int position = -1;
     int64_t slot = 0;
-    const int s = token < a.batch.tokens ? paged_sequence_of(a.batch, token) : -1;
+    PagedSequence seq{0, 0, 0};
+    const int s = token < a.batch.tokens ? paged_sequence_of(a.batch, token, a.status, seq) : -1;
     if (s >= 0) {
-      const PagedSequence seq = paged_sequence(a.batch, s, a.status);
-      const int row = token - seq.q_begin;
-      if (row >= 0 && row < seq.q_len) {
-        position = seq.kv_len - seq.q_len + row;
-        if (position >= 0 && a.rotary_dim > 0 && position >= a.table_positions) {
-          report_status(a.status, kStatusPositionOutOfRange);
+      position = seq.kv_len - seq.q_len + token - seq.q_begin;
+      if (position >= 0 && a.rotary_dim > 0 && position >= a.table_positions) {
+        report_status(a.status, kStatusPositionOutOfRange);
+        position = -1;
+      }
+      if (position >= 0) {
+        const int index = position >> a.cache.page_shift;
+        const int page = __ldcg(a.batch.page_table + static_cast<int64_t>(s) * a.batch.table_stride + index);
+        if (page >= 0 && page < a.cache.page_count) {
+          const int in_page = position & ((1 << a.cache.page_shift) - 1);
+          slot = (static_cast<int64_t>(page) * a.cache.kv_heads << a.cache.page_shift) + in_page;
+        } else {
+          report_status(a.status, kStatusPagedBatch);
           position = -1;
-        }
-        if (position >= 0) {
-          const int index = position >> a.cache.page_shift;
-          const int page = __ldcg(a.batch.page_table + static_cast<int64_t>(s) * a.batch.table_stride + index);
-          if (page >= 0 && page < a.cache.page_count) {
-            const int in_page = position & ((1 << a.cache.page_shift) - 1);
-            slot = (static_cast<int64_t>(page) * a.cache.kv_heads << a.cache.page_shift) + in_page;
-          } else {
-            report_status(a.status, kStatusPagedBatch);
-            position = -1;
-          }
         }
       }
     }
