@@ -383,14 +383,14 @@ __global__ void __launch_bounds__(FewShared<kDim>::kThreads, FewShared<kDim>::kC
           }
         }
       }
-      // The reference moves only when a score exceeds it by more than the threshold, so probabilities
-      // stay below 2^8; the row's maximum is only looked for then.
+      // The reference moves only when a score exceeds it by more than the threshold (rounded down, so that
+      // none passes further), so probabilities stay below 2^8; the row's maximum is only looked for then.
       float top[2];
       bool move = false;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         top[e] = fmaxf(fmaxf(x[0][2 * e], x[0][2 * e + 1]), fmaxf(x[1][2 * e], x[1][2 * e + 1]));
-        move |= top[e] > reference[e] + kRescaleThreshold || (reference[e] == -INFINITY && top[e] != -INFINITY);
+        move |= top[e] > __fadd_rd(reference[e], kRescaleThreshold);
       }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll

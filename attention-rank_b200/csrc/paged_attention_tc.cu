@@ -557,9 +557,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const float block_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
-        // the row's reference moves only when the block's maximum exceeds it by more than the threshold,
-        // so probabilities stay below 2^8 and O is rarely rescaled
-        const bool move = block_top > reference + kRescaleThreshold || (reference == -INFINITY && block_top != -INFINITY);
+        // the row's reference moves only when the block's maximum exceeds it by more than the threshold
+        // (rounded down, so that none passes further), so probabilities stay below 2^8 and O is rarely rescaled
+        const bool move = block_top > __fadd_rd(reference, kRescaleThreshold);
         const bool rescale = move && reference != -INFINITY;
         if (__any_sync(0xffffffffu, rescale)) {
           // O holds the segment's blocks before this one
