@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -108,6 +109,17 @@ cudaError_t launch_paged_attention_chunk(const PagedAttentionArgs& args, int few
 
 // ------------------------------------------------------------------------------ device helpers
 #ifdef __CUDACC__
+
+// The probabilities 2^(x - reference) are rounded to the 16-bit type for the product with V: the tensor
+// cores take both operands in one type, and two products for a split probability would double the work.
+// A row's reference is set kReferenceBelow under its maximum and moves when a score exceeds it by more than
+// kReferenceReach, so a probability stays below 2^15 in fp16 and 2^8 in bf16. In fp16 that leaves weights
+// down to 2^-21 of the largest one with all their bits; with a reference at the maximum itself it was 2^-14,
+// and 2^17 keys of 2^-25.5 each, 1/362 of the row together, vanished.
+template <typename T>
+constexpr float kReferenceBelow = std::is_same_v<T, __half> ? 7.0f : 0.0f;  // log2 units
+template <typename T>
+constexpr float kReferenceReach = kReferenceBelow<T> + 8.0f;
 
 // The batch's arrays are read through L2 (__ldcg): a kernel launched ahead of its producer's end must not
 // find an older copy of them in the read-only cache.

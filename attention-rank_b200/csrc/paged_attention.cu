@@ -35,7 +35,6 @@ using namespace async;
 constexpr int kBlock = 64;          // keys a block
 constexpr int kRows = 16;           // rows a tile
 constexpr int kCombineThreads = 256;
-constexpr float kRescaleThreshold = 8.0f;  // log2 units
 
 // One (sequence, KV head, 16 rows) of the line of work.
 struct FewTile {
@@ -383,23 +382,24 @@ __global__ void __launch_bounds__(FewShared<kDim>::kThreads, FewShared<kDim>::kC
           }
         }
       }
-      // The reference moves only when a score exceeds it by more than the threshold (rounded down, so that
-      // none passes further), so probabilities stay below 2^8; the row's maximum is only looked for then.
+      // The reference moves only when a score exceeds it by more than its reach (rounded down, so that none
+      // passes further); the row's maximum is only looked for then.
       float top[2];
       bool move = false;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         top[e] = fmaxf(fmaxf(x[0][2 * e], x[0][2 * e + 1]), fmaxf(x[1][2 * e], x[1][2 * e + 1]));
-        move |= top[e] > __fadd_rd(reference[e], kRescaleThreshold);
+        move |= top[e] > __fadd_rd(reference[e], kReferenceReach<T>);
       }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
           top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-          if (top[e] > reference[e]) {
-            const float factor = reference[e] == -INFINITY ? 0.0f : ex2_ftz(reference[e] - top[e]);
-            reference[e] = top[e];
+          const float moved = top[e] - kReferenceBelow<T>;
+          if (moved > reference[e]) {
+            const float factor = reference[e] == -INFINITY ? 0.0f : ex2_ftz(reference[e] - moved);
+            reference[e] = moved;
             l[e] *= factor;
 #pragma unroll
             for (int d = 0; d < kDim / 8; ++d) {

@@ -49,7 +49,6 @@ constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kTmemO = 256;
 constexpr int kJoinThreads = 256;
 constexpr int kJoinRows = 32;                       // rows of a tile that one joining CTA takes
-constexpr float kRescaleThreshold = 8.0f;           // log2 units
 constexpr int kChains = 4;                          // independent accumulators per row reduction
 
 struct __align__(16) Control {
@@ -557,15 +556,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const float block_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
-        // the row's reference moves only when the block's maximum exceeds it by more than the threshold
-        // (rounded down, so that none passes further), so probabilities stay below 2^8 and O is rarely rescaled
-        const bool move = block_top > __fadd_rd(reference, kRescaleThreshold);
+        // the row's reference moves only when the block's maximum exceeds it by more than its reach (rounded
+        // down, so that no score passes further), so O is rarely rescaled
+        const bool move = block_top > __fadd_rd(reference, kReferenceReach<T>);
+        const float moved = block_top - kReferenceBelow<T>;
         const bool rescale = move && reference != -INFINITY;
         if (__any_sync(0xffffffffu, rescale)) {
           // O holds the segment's blocks before this one
           wait(ctl.o_full[half], (outputs - 1) & 1);
           fence_after();
-          const float factor = rescale ? ex2_ftz(reference - block_top) : 1.0f;
+          const float factor = rescale ? ex2_ftz(reference - moved) : 1.0f;
 #pragma unroll 1
           for (int i = 0; i < kDim / 32; ++i) {
             uint32_t raw[32];
@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           l *= factor;
         }
-        if (move) reference = block_top;
+        if (move) reference = moved;
         const float base = reference == -INFINITY ? 0.0f : -reference;
         const unsigned long long scale2 = pack_f32x2(a.scale_log2, a.scale_log2);
         const unsigned long long base2 = pack_f32x2(base, base);
