@@ -17,6 +17,11 @@ void require(bool ok, const char* who, const char* what) {
 }
 
 bool aligned16(const void* pointer) { return (reinterpret_cast<uintptr_t>(pointer) & 15) == 0; }
+bool aligned4(const void* pointer) { return (reinterpret_cast<uintptr_t>(pointer) & 3) == 0; }
+
+void check_status_word(const char* who, const int* device_status) {
+  require(aligned4(device_status), who, "device_status must be 4-byte aligned");
+}
 
 // Makes the device that holds `array` current for the call, so that a call on another device's
 // arrays and stream runs there. Asking the stream instead is not allowed while it is captured.
@@ -116,6 +121,8 @@ arb::PagedBatch checked_batch(const char* who, const ar_paged_batch* batch, cons
   if (batch->sequence_count > 0) {
     require(batch->q_offsets != nullptr && batch->kv_lengths != nullptr && batch->page_table != nullptr, who,
             "null batch array");
+    require(aligned4(batch->q_offsets) && aligned4(batch->kv_lengths) && aligned4(batch->page_table), who,
+            "q_offsets, kv_lengths and page_table must be 4-byte aligned");
   }
   arb::PagedBatch out;
   out.sequences = batch->sequence_count;
@@ -156,6 +163,8 @@ int attention_call(const char* who, const ar_paged_cache* cache, const ar_paged_
   require(q != nullptr && out != nullptr && aligned16(q) && aligned16(out), who,
           "q and out must be 16-byte aligned device arrays");
   require(q != out, who, "out must not overlap q");
+  require(aligned4(lse), who, "lse must be 4-byte aligned");
+  check_status_word(who, device_status);
   const int64_t needed = arb::paged_attention_workspace(args.cache, args.batch, query_heads);
   if (needed > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < needed)) {
     throw arb::Error(std::string(who) + ": needs a 16-byte aligned workspace of " + std::to_string(needed) + " bytes");
@@ -229,6 +238,9 @@ int ar_rotary_positions(const void* x, int64_t x_token_stride, int64_t x_head_st
             "null argument");
     require(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 1) == 0, who,
             "x and out must be aligned to their type");
+    require(aligned4(positions) && aligned4(cos_table) && aligned4(sin_table), who,
+            "positions and the tables must be 4-byte aligned");
+    check_status_word(who, device_status);
     require(x_head_stride >= 0 && x_token_stride >= 0, who, "strides must not be negative");
     require((heads == 1 || out_head_stride >= head_dim) && (token_count == 1 || out_token_stride >= head_dim), who,
             "out's strides must be at least head_dim, or its rows would overlap");
@@ -291,6 +303,7 @@ int ar_paged_append(const ar_paged_cache* cache, const ar_paged_batch* batch, co
     if (args.batch.tokens == 0 || args.batch.sequences == 0) return AR_OK;
     require(qkv != nullptr && aligned16(qkv), who, "qkv must be a 16-byte aligned device array");
     require(bias == nullptr || aligned16(bias), who, "bias must be 16-byte aligned");
+    check_status_word(who, device_status);
     args.qkv = qkv;
     args.qkv_stride = qkv_stride;
     args.bias = bias;

@@ -308,7 +308,7 @@ int ar_decode_attention(const void* q, const void* k_cache, const void* v_cache,
  * per prompt and rotates with one unscaled table (kernels.cu:85-115, model.cu:426-440). They let
  * many prompts be prefilled in chunks and answered together. Device pointers, asynchronous on
  * `stream`; a call runs on the device that holds its arrays, whichever is current (stream NULL: that
- * device's default stream). No call allocates or synchronises, so every one may be captured into a
+ * device's default stream). Arrays are aligned to their type at least. No call allocates or synchronises, so every one may be captured into a
  * CUDA graph; lengths, offsets and page ids are read on the device when the work runs.
  * ------------------------------------------------------------------------------------------ */
 
