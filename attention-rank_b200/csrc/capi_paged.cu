@@ -1,5 +1,6 @@
 // extern "C" entry points of the serving operators (declarations in include/attnrank_b200.h): every
 // argument is checked on the host before any device work.
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -21,6 +22,24 @@ bool aligned4(const void* pointer) { return (reinterpret_cast<uintptr_t>(pointer
 
 void check_status_word(const char* who, const int* device_status) {
   require(aligned4(device_status), who, "device_status must be 4-byte aligned");
+}
+
+// Do any two of the rows [t * token_stride + h * head_stride, .. + head_dim), t < tokens, h < heads, share
+// an element? Both strides are at least head_dim where there is more than one row along them.
+bool rows_overlap(int64_t tokens, int64_t token_stride, int64_t heads, int64_t head_stride, int64_t head_dim) {
+  using Wide = __int128;
+  if (tokens == 1 || heads == 1 || Wide(heads - 1) * head_stride + head_dim <= token_stride ||
+      Wide(tokens - 1) * token_stride + head_dim <= head_stride) {
+    return false;  // the usual layouts: heads inside a token, or tokens inside a head
+  }
+  for (int64_t h = 1; h < heads; ++h) {  // rows h heads apart: the nearest multiples of token_stride
+    const Wide apart = Wide(h) * head_stride;
+    const Wide below = std::min<Wide>(apart / token_stride, tokens - 1);
+    const Wide above = std::min<Wide>(below + 1, tokens - 1);
+    if (apart - below * token_stride < head_dim) return true;
+    if (above * token_stride - apart < head_dim && apart - above * token_stride < head_dim) return true;
+  }
+  return false;
 }
 
 // Makes the device that holds `array` current for the call, so that a call on another device's
@@ -240,12 +259,14 @@ int ar_rotary_positions(const void* x, int64_t x_token_stride, int64_t x_head_st
             "x and out must be aligned to their type");
     require(aligned4(positions) && aligned4(cos_table) && aligned4(sin_table), who,
             "positions and the tables must be 4-byte aligned");
-    check_status_word(who, device_status);
     require(x_head_stride >= 0 && x_token_stride >= 0, who, "strides must not be negative");
     require((heads == 1 || out_head_stride >= head_dim) && (token_count == 1 || out_token_stride >= head_dim), who,
             "out's strides must be at least head_dim, or its rows would overlap");
+    require(!rows_overlap(token_count, out_token_stride, heads, out_head_stride, head_dim), who,
+            "out's strides would make its rows overlap");
     require(out != x || (out_token_stride == x_token_stride && out_head_stride == x_head_stride), who,
             "in place needs x's strides");
+    check_status_word(who, device_status);
     arb::RotaryArgs args;
     args.x = x;
     args.x_token_stride = x_token_stride;

@@ -308,8 +308,9 @@ int ar_decode_attention(const void* q, const void* k_cache, const void* v_cache,
  * per prompt and rotates with one unscaled table (kernels.cu:85-115, model.cu:426-440). They let
  * many prompts be prefilled in chunks and answered together. Device pointers, asynchronous on
  * `stream`; a call runs on the device that holds its arrays, whichever is current (stream NULL: that
- * device's default stream). Arrays are aligned to their type at least. No call allocates or synchronises, so every one may be captured into a
- * CUDA graph; lengths, offsets and page ids are read on the device when the work runs.
+ * device's default stream). Arrays are aligned to their type at least. No call allocates or
+ * synchronises, so every one may be captured into a CUDA graph; lengths, offsets and page ids are read
+ * on the device when the work runs.
  * ------------------------------------------------------------------------------------------ */
 
 /* How the frequencies theta^(-2i/r), i < r/2, r = rotary_dim, are stretched for contexts longer
@@ -352,10 +353,11 @@ int ar_rope_table_scaled(const ar_rope_scaling* scaling, int positions, float* c
  * strides in elements) by its token's position: the pair (a, b) becomes (a c - b s, b c + a s),
  * where (a, b) are values (i, i + rotary_dim / 2), or (2i, 2i + 1) when `interleaved`. `inverse`
  * rotates back, which is also the gradient with respect to x. The other values are copied. out has
- * its own strides; out == x with x's strides works in place, any other overlap is undefined. A
- * position outside [0, table_positions) sets *device_status (nullable) to 2 and leaves its token's
- * rows of out as they were. rotary_dim is even, 2..head_dim, head_dim <= 1024, heads <= 65536,
- * positions int32 [token_count], tables fp32 [table_positions, rotary_dim / 2]. Arithmetic in fp32, one rounding. */
+ * its own strides, under which no two of its rows overlap; out == x with x's strides works in place,
+ * any other overlap is undefined. A position outside [0, table_positions) sets *device_status
+ * (nullable) to 2 and leaves its token's rows of out as they were. rotary_dim is even, 2..head_dim,
+ * head_dim <= 1024, heads <= 65536, positions int32 [token_count], tables fp32 [table_positions,
+ * rotary_dim / 2]. Arithmetic in fp32, one rounding. */
 int ar_rotary_positions(const void* x, int64_t x_token_stride, int64_t x_head_stride, void* out,
                         int64_t out_token_stride, int64_t out_head_stride, const int32_t* positions, int token_count,
                         int heads, int head_dim, int rotary_dim, int interleaved, int inverse, const float* cos_table,

@@ -48,3 +48,36 @@ def test_status_words_and_lse_are_aligned(off):
     for lse, status, message in ((ADDRESS + off, None, "lse"), (None, ADDRESS + off, "device_status")):
         refused(lib.ar_paged_attention(cache, batch, a["q"], a["q_stride"], a["heads"], a["scale"], a["window"], a["out"],
                                        a["out_stride"], lse, a["workspace"], a["bytes"], status, None), message)
+
+
+def share_elements(tokens, token_stride, heads, head_stride, head_dim):
+    seen = set()
+    for t in range(tokens):
+        for h in range(heads):
+            row = range(t * token_stride + h * head_stride, t * token_stride + h * head_stride + head_dim)
+            if not seen.isdisjoint(row):
+                return True
+            seen.update(row)
+    return False
+
+
+def test_rotary_output_rows_never_overlap():
+    """Every stride pair of small shapes against the elements themselves: refused where two rows share
+    one. The others fail a later check here (the status word), so that no call reaches a device."""
+    outcomes = set()
+    for head_dim in (2, 3, 5):
+        for tokens in (1, 2, 3, 7):
+            for heads in (1, 2, 3, 4):
+                for ot in range(head_dim, 5 * head_dim + 2):
+                    for oh in range(head_dim, 5 * head_dim + 2):
+                        code = rotary(dict(tokens=tokens, heads=heads, head_dim=head_dim, rotary=2, ot=ot, oh=oh), status=ADDRESS + 1)
+                        overlap = share_elements(tokens, ot, heads, oh, head_dim)
+                        refused(code, "rows overlap" if overlap else "device_status")
+                        outcomes.add(overlap)
+    assert outcomes == {True, False}
+
+
+@pytest.mark.parametrize("change", [dict(tokens=2**31 - 1, ot=2**62, oh=128), dict(tokens=2**31 - 1, ot=128, oh=2**62),
+                                    dict(tokens=1, heads=65536, ot=0, oh=2**47)])
+def test_large_strides_do_not_overflow_the_check(change):
+    refused(rotary(change, status=ADDRESS + 1), "device_status")
