@@ -220,9 +220,9 @@ void launch_layout(const RotaryArgs& a, cudaStream_t stream) {
     const int groups = (a.heads + heads_per_item - 1) / heads_per_item;
     const int64_t per_token = static_cast<int64_t>(groups) * units;
     const int step = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(a.tokens, (int64_t{1} << 30) / per_token)));
-    for (int begin = 0; begin < a.tokens; begin += step) {  // one launch but for batches beyond 2^30 items
+    for (int64_t begin = 0; begin < a.tokens; begin += step) {  // one launch but for batches beyond 2^30 items
       RotaryArgs part = a;
-      part.tokens = std::min(step, a.tokens - begin);
+      part.tokens = static_cast<int>(std::min<int64_t>(step, a.tokens - begin));
       part.x = static_cast<const T*>(a.x) + begin * a.x_token_stride;
       part.out = static_cast<T*>(a.out) + begin * a.out_token_stride;
       part.positions = a.positions + begin;
