@@ -135,6 +135,7 @@ arb::PagedBatch checked_batch(const char* who, const ar_paged_batch* batch, cons
   require(batch != nullptr, who, "null batch");
   require(batch->sequence_count >= 0 && batch->token_count >= 0, who,
           "sequence_count and token_count must not be negative");
+  require(batch->sequence_count <= 1 << 30, who, "sequence_count must be at most 2^30");
   require(batch->max_query_tokens > 0, who, "max_query_tokens must be positive");
   require(batch->page_table_stride > 0, who, "page_table_stride must be positive");
   if (batch->sequence_count > 0) {

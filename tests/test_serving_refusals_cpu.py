@@ -81,3 +81,11 @@ def test_rotary_output_rows_never_overlap():
                                     dict(tokens=1, heads=65536, ot=0, oh=2**47)])
 def test_large_strides_do_not_overflow_the_check(change):
     refused(rotary(change, status=ADDRESS + 1), "device_status")
+
+
+def test_sequence_counts_whose_indexes_would_overflow_are_refused():
+    for call in (append, attention):
+        refused(call(dict(sequences=(1 << 30) + 1)), "2^30")
+        refused(call(dict(sequences=2**31 - 1)), "2^30")
+    assert lib.ar_paged_attention_workspace(*descriptors(dict(sequences=2**31 - 1)), 28) == -1
+    assert lib.ar_paged_attention_workspace(*descriptors(dict(sequences=1 << 30)), 28) > 0
