@@ -11,6 +11,7 @@
 // order of multiplies), only the storage type of activations changes from fp32 to 16 bits (T =
 // __half, the default, or __nv_bfloat16).
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "layer_kernels.h"
@@ -374,14 +375,16 @@ int row_threads(int hidden, int* vpt) {
 }  // namespace
 
 int sm_count() {
-  static int cached = 0;
-  if (cached == 0) {
+  static std::atomic<int> cached{0};  // host threads may ask at once
+  int count = cached.load(std::memory_order_relaxed);
+  if (count == 0) {
     int device = 0;
     cudaGetDevice(&device);
-    cudaDeviceGetAttribute(&cached, cudaDevAttrMultiProcessorCount, device);
-    if (cached <= 0) cached = 148;
+    cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device);
+    if (count <= 0) count = 148;
+    cached.store(count, std::memory_order_relaxed);
   }
-  return cached;
+  return count;
 }
 
 // CTAs of `kernel` that fit on one SM at `threads` threads (registers and shared memory decide).

@@ -23,6 +23,7 @@
 
 #include "async_copy.cuh"
 #include "common.cuh"
+#include "device_once.h"
 #include "layer_kernels.h"
 #include "paged.h"
 #include "paged_plan.cuh"
@@ -648,14 +649,12 @@ cudaError_t launch_few(const PagedAttentionArgs& a, int most, cudaStream_t strea
   static_assert(Shared::kCtasPerSm * (Shared::bytes() + 1024) <= 228 * 1024, "the CTAs of an SM share its shared memory");
   int device = 0;
   cudaGetDevice(&device);
-  static uint64_t configured = 0;  // the shared-memory opt-in is a per-device attribute
-  if (device >= 64 || !(configured & (1ull << device))) {
-    const cudaError_t status =
-        cudaFuncSetAttribute(paged_attention_few_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(Shared::bytes()));
-    if (status != cudaSuccess) return status;
-    if (device < 64) configured |= 1ull << device;
-  }
+  static DeviceOnce configured;  // the shared-memory opt-in is a per-device attribute
+  const cudaError_t opted = configured.run(device, [] {
+    return cudaFuncSetAttribute(paged_attention_few_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(Shared::bytes()));
+  });
+  if (opted != cudaSuccess) return opted;
   CUtensorMap k_map, v_map;
   const int rows = std::min(1 << a.cache.page_shift, kBlock);
   if (!encode_pages<T>(&k_map, a.cache, a.cache.k_pages, rows) ||

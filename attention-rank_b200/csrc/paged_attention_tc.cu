@@ -30,6 +30,7 @@
 
 #include "async_copy.cuh"
 #include "common.cuh"
+#include "device_once.h"
 #include "layer_kernels.h"
 #include "paged.h"
 #include "paged_plan.cuh"
@@ -802,14 +803,12 @@ cudaError_t launch_chunk(const PagedAttentionArgs& a, int few, cudaStream_t stre
   static_assert(Layout<kDim>::bytes() <= 227 * 1024, "one CTA's shared memory");
   int device = 0;
   cudaGetDevice(&device);
-  static uint64_t configured = 0;  // the shared-memory opt-in is a per-device attribute
-  if (device >= 64 || !(configured & (1ull << device))) {
-    const cudaError_t status =
-        cudaFuncSetAttribute(paged_attention_chunk_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(Layout<kDim>::bytes()));
-    if (status != cudaSuccess) return status;
-    if (device < 64) configured |= 1ull << device;
-  }
+  static DeviceOnce configured;  // the shared-memory opt-in is a per-device attribute
+  const cudaError_t opted = configured.run(device, [] {
+    return cudaFuncSetAttribute(paged_attention_chunk_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(Layout<kDim>::bytes()));
+  });
+  if (opted != cudaSuccess) return opted;
   const int group = a.query_heads / a.cache.kv_heads;
   ChunkArgs c;
   c.a = a;
