@@ -89,3 +89,21 @@ def test_sequence_counts_whose_indexes_would_overflow_are_refused():
         refused(call(dict(sequences=2**31 - 1)), "2^30")
     assert lib.ar_paged_attention_workspace(*descriptors(dict(sequences=2**31 - 1)), 28) == -1
     assert lib.ar_paged_attention_workspace(*descriptors(dict(sequences=1 << 30)), 28) > 0
+
+
+@pytest.mark.parametrize("heads,kv_heads,head_dim,most", [(28, 4, 128, 1), (32, 8, 128, 4096), (128, 1, 64, 7), (5, 5, 64, 300)])
+def test_workspace_does_not_depend_on_the_batch_and_is_required_whole(heads, kv_heads, head_dim, most):
+    """One size for any number of sequences and rows that reach the bound, and for its wider pools; a byte
+    less, a misaligned address or none is refused."""
+    shape = dict(kv_heads=kv_heads, head_dim=head_dim, most=most)
+    sizes = {lib.ar_paged_attention_workspace(*descriptors({**shape, **more}), heads)
+             for more in (dict(sequences=1, tokens=most), dict(sequences=500, tokens=5000), dict(sequences=500, tokens=5000, pages=99, stride=70))}
+    assert len(sizes) == 1
+    needed = sizes.pop()
+    assert 0 < needed <= 64 << 20
+    row = heads * head_dim
+    call = dict(**shape, heads=heads, q_stride=row, out_stride=row, sequences=500, tokens=5000)
+    refused(attention({**call, "bytes": needed - 1}), f"workspace of {needed} bytes")
+    refused(attention({**call, "bytes": 0}), "workspace")
+    refused(attention({**call, "workspace": ADDRESS + 8, "bytes": needed}), "workspace")
+    refused(attention({**call, "workspace": None, "bytes": needed}), "workspace")
