@@ -6,7 +6,7 @@
 //
 // Few rows a KV head (single tokens, a few drafted ones: at most 48 rows of new tokens x query heads
 // of the group): every K and V value is used once to three times per call, so HBM bounds the kernel (64
-// single tokens over up to 8K keys, 1.24 GB: 191 us, 0.98 of the measured copy). K and V arrive
+// single tokens over up to 8K keys, 1.24 GB: 196 to 201 us, 0.94 to 0.96 of the measured copy). K and V arrive
 // in 64-key blocks by TMA (192 KB of ring per SM, above the 45 KB that 6.5 TB/s x 1 us of latency
 // needs), and the products run on mma.sync m16n8k16 with the group's rows as its 16 rows: the 128 rows
 // of a tcgen05 tile would be 7/8 empty.
@@ -16,6 +16,8 @@
 // its rows, the others write fp32 partial sums that the second kernel joins in order. Every CTA finds
 // its part from q_offsets and kv_lengths itself, so no plan is made on the host and a captured graph
 // follows the lengths it finds.
+// Every mbarrier wait is bounded; a warp whose wait gives up records kStatusWaitTimeout and meets the others at
+// the barriers of the rest of its part without computing, and the loading warp leaves after its last copies.
 // More rows: paged_attention_tc.cu.
 #include <algorithm>
 #include <cmath>
@@ -86,7 +88,7 @@ struct FewShared {
   int poison[2];  // of this segment and the next, in turn
   PlanScratch<kThreads> plan;
   float2 stats[4][kRows];
-  alignas(16) float merge[4][kRows][kPad];
+  alignas(16) float merge[4][kRows][kPad];  // read as float4
   static constexpr size_t bytes() { return 2 * kStages * kBlockBytes + sizeof(FewShared) + 1024; }
 };
 
@@ -419,7 +421,7 @@ __global__ void __launch_bounds__(FewShared<kDim>::kThreads, FewShared<kDim>::kC
           const float p0 = ex2_ftz(x[n][2 * e] - base);
           const float p1 = ex2_ftz(x[n][2 * e + 1] - base);
           l[e] += p0 + p1;
-          p[2 * n + e] = pack2<T>(p0, p1);
+          p[2 * n + e] = pack2<T>(p0, p1);  // rounded: see kReferenceBelow
         }
       }
       const int stage = turn % kStages;
@@ -674,9 +676,19 @@ cudaError_t launch_few(const PagedAttentionArgs& a, int most, cudaStream_t strea
 // where a 256-row tile of the chunk kernel would be nearly empty; the others to the chunk kernel. Only
 // what the bound on the new tokens allows for is launched, and a batch of one sequence with a larger
 // bound takes the chunk kernel alone: the launches it would save cost more than a short chunk there.
-// Both forms at 7 heads a KV head, this one first: 6 tokens (42 rows), one sequence over 4K keys 18.3 and
-// 34.0 us, 16 sequences over 512 keys 20.1 and 25.5, over 4K keys 59.9 and 55.6; 9 tokens (63 rows), 16
-// sequences over 4K keys 74.1 and 58.6.
+// Both forms, this one first, in us a call in a graph (head_dim 128, fp16, the cache partly in L2):
+//   heads x KV heads   rows   1 x 4K keys    16 x 512 keys   16 x 4K keys    64 x 1000 keys
+//   7 x 4              28     27.0 / 38.0    18.6 / 19.4     44.4 / 41.9     57.5 / 43.5
+//                      42     22.7 / 35.8    20.3 / 19.6     59.7 / 41.8     76.2 / 43.5
+//                      63     21.4 / 36.7    23.0 / 19.8     68.9 / 42.6     95.3 / 44.0
+//   8 x 4              48     20.1 / 32.9    19.8 / 19.3     59.0 / 41.3     75.2 / 44.0
+//   4 x 8              28     22.2 / 31.4    22.4 / 22.5     72.4 / 65.9     106.6 / 78.3
+//                      48     22.1 / 34.2    27.8 / 22.5     136.0 / 68.2    145.0 / 74.3
+//   1 x 16             28     20.7 / 25.0    35.2 / 33.4     175.2 / 121.3   212.1 / 165.5
+//                      48     23.6 / 25.4    49.5 / 33.6     261.0 / 132.3   306.3 / 165.9
+// The rule looks at rows alone. That is right for one sequence, and for single tokens, where this kernel is at
+// HBM's rate; for many sequences of 28 to 48 rows the chunk kernel is the faster one, most where no heads are
+// shared and the cache is long.
 constexpr int kFewRows = 48;
 
 struct FormChoice {

@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             p0 = ex2_ftz(p0);
             p1 = ex2_ftz(p1);
             sums[i % (kChains / 2)] = add_f32x2(sums[i % (kChains / 2)], pack_f32x2(p0, p1));
-            packed[i] = pack2<T>(p0, p1);
+            packed[i] = pack2<T>(p0, p1);  // rounded: see kReferenceBelow
           }
           tmem_st16(s_tmem + column, packed);
         };

@@ -5,12 +5,13 @@
 // digits of the fraction near 2^24 turns and is off by 1e-3 rad at 1e4) and split there into its
 // nearest whole number n of quarters and the remainder u in [-1/2, 1/2]; sin and cos of pi/2 u are
 // polynomials in fp32, n's low bits swap them and give their signs. A thread keeps its column's
-// frequency and walks down the positions, so a value costs five fp64 and about twenty fp32 operations:
-// bound by the 8 bytes it writes: 128K positions x 32 pairs take 10.4 us timed alone with a cold cache
-// (33.5 MB, 0.5 of the measured copy; 12.9 us with sincospi of the fp32 remainder).
+// frequency and walks down the positions, so a value costs five fp64 and about twenty other operations.
+// Their issue bounds it, not the 8 bytes a value, which stay in L2: 128K positions x 32 pairs (33.5 MB) take
+// 10.2 us a call, half of the measured copy, with 73% of the issue slots used, the integer and logic pipe 55%
+// busy and fp64 11% (12.9 us with sincospi of the fp32 remainder in place of the polynomials).
 //
 // Rotation: y_a = a c - b s, y_b = b c + a s, one read and one write of each 16-bit value: HBM bounds
-// it (16K tokens x 32 heads x 128, half of each head: 46.5 us a call, 0.89 of the measured copy).
+// it (16K tokens x 32 heads x 128, half of each head: 45.3 to 46.6 us a call, 0.89 to 0.91 of the measured copy).
 #include <algorithm>
 
 #include "common.cuh"
@@ -23,8 +24,10 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kTableUnroll = 2;  // positions a thread computes before it stores
 
-// (sin, cos) of `quarter` quarter turns. The polynomials have the least largest error on [-1/2, 1/2]:
-// 1.2e-9 for sin, 5e-11 for cos; 9.4e-8 and 5.8e-8 with the fp32 roundings, checked at 2 million points.
+// (sin, cos) of `quarter` quarter turns. The polynomials have the least largest error on [-1/2, 1/2] (Remez
+// exchange): 1.2e-9 for sin, 5.4e-11 for cos; 3.0e-8 and 6.7e-9 with the coefficients rounded to fp32, 1.1e-7 and
+// 7.5e-8 with the roundings of u and of each step, checked at 44 million points. That is 1.5 times the error of
+// an fp64 value rounded once, chosen for the time above.
 __device__ __forceinline__ void sincos_quarters(double quarter, float& s, float& c) {
   const double shifted = quarter + 6755399441055744.0;  // 1.5 x 2^52: the sum's low bits hold the nearest integer
   const int n = __double2loint(shifted);
@@ -143,7 +146,10 @@ __global__ void __launch_bounds__(kThreads) rotary_positions_kernel(const Rotary
 }
 
 // Form for sizes, strides or addresses that do not hold 16-byte accesses: an item is one token,
-// kHeads heads and one rotation pair, or two values behind the rotated part.
+// kHeads heads and one rotation pair, or two values behind the rotated part. Its accesses of 2 bytes bound
+// it, a warp's being 64 neighbouring bytes in the half layout and every other value, twice, interleaved: 16K
+// tokens x 32 heads x 128 take 102 us with 66 values rotated (half) and 88 us with 126 (interleaved), against
+// 49 us in the vector form with 64 or 128 and a floor of 41 us; cold cache, timed alone.
 template <typename T, bool kInterleaved, int kHeads>
 __global__ void __launch_bounds__(kThreads) rotary_positions_pairs_kernel(const RotaryArgs a, int units,
                                                                           int rotated_units, int groups,
