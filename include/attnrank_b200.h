@@ -384,10 +384,10 @@ typedef struct {
  * page_table_stride]; sequence_count is at most 2^30. token_count is the number of rows in the call's
  * buffers, max_query_tokens a bound on the new tokens of any sequence. A sequence with decreasing
  * offsets, rows past token_count, more new tokens than max_query_tokens, or a length that is negative
- * or beyond its page table's row sets *device_status (nullable) to 4 and is left out; a needed page id
- * outside [0, page_count) sets it too (what is computed from that page is unspecified; nothing outside
- * the arrays is touched). What becomes of a row that two sequences claim is unspecified. A status word
- * keeps its first value until the caller clears it. */
+ * or beyond its page table's row (or 2^31 - 1025) sets *device_status (nullable) to 4 and is left out;
+ * a needed page id outside [0, page_count) sets it too (what is computed from that page is unspecified;
+ * nothing outside the arrays is touched). What becomes of a row that two sequences claim is unspecified.
+ * A status word keeps its first value until the caller clears it. */
 typedef struct {
   int sequence_count;
   int token_count;
